@@ -1,0 +1,380 @@
+"""Workloads of the 8-bit integer and grouped matrix products, as programs that use this package call them.
+
+Three operators, each with the calls that go with it in a serving step:
+
+``linear``   a dense product in 8-bit integers: bf16 tokens are quantised (one scale per token) and multiplied with
+             int8 weights (one scale per output channel): ``act_quant_int8`` and ``matmul_int8``.
+``grouped``  the products of one expert layer, each expert's matrix with the ragged set of rows that was routed to
+             it: ``group_routes`` and ``grouped_matmul``, bf16 or int8, optionally with SwiGLU on a gate/up matrix
+             or with router weights on the rows.  Rows come as tokens with their top-k ids, or already laid out by
+             expert, as an expert-parallel rank receives them.
+``experts``  a whole expert layer with an int8 bank: ``experts_int8``.
+
+The sizes are those of the configurations this repository is benchmarked and tested on (hidden 1024 to 7168,
+intermediate 512 to 2048, 16 to 256 experts, top-2 to top-8).  ``draw()`` takes rows from one token to thousands,
+depths that are any multiple of 16, any number of output channels, even and skewed routings, padded batches.
+
+Definitions.  A row of activations with largest magnitude a is held as q = round(127 x / a), ties to even, with the
+scale a / 127 (a row of zeros: zeros).  SwiGLU is silu(gate) * up of the products; between an expert's two products
+the activations are bf16, and quantised from there like any other row.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+own = False
+
+DEV = "cuda"
+
+
+def listed():
+    return [
+        # one user's token through a shared expert's gate/up matrix (hidden 7168, intermediate 2048): the stream of
+        # the weights and two launches
+        dict(name="linear_1", op="linear", M=1, N=4096, K=7168, out="bf16"),
+        # a decode batch through the same expert's down matrix
+        dict(name="linear_48", op="linear", M=48, N=7168, K=2048, out="bf16"),
+        # a prompt chunk of odd length, kept in float32 for what follows
+        dict(name="linear_513_f32", op="linear", M=513, N=5120, K=1536, out="f32"),
+        # a full prefill batch
+        dict(name="linear_8192", op="linear", M=8192, N=4096, K=7168, out="bf16"),
+        # four sequences decoding on a bf16 layer: 32 rows, about 28 of 128 experts, SwiGLU fused
+        dict(name="grouped_bf16_4", op="grouped", fmt="bf16", M=4, k=8, E=128, K=2048, N=768, act=True, weigh=False,
+             skew=0.0),
+        # an expert-parallel rank's share of a decode step: 300 rows laid out over 64 experts
+        dict(name="grouped_int8_rank_300", op="grouped", fmt="int8", M=300, k=0, E=64, K=7168, N=2048, act=True,
+             weigh=False, skew=0.0),
+        # a long prompt on the bf16 layer, the down products with their router weights
+        dict(name="grouped_bf16_4096", op="grouped", fmt="bf16", M=4096, k=8, E=128, K=768, N=2048, act=False,
+             weigh=True, skew=0.0),
+        # a prompt of 1500 tokens on a layer of 160 experts, skewed: experts of a thousand rows beside nearly empty ones
+        dict(name="grouped_int8_1500", op="grouped", fmt="int8", M=1500, k=8, E=160, K=1536, N=5120, act=False,
+             weigh=True, skew=0.7),
+        # a small layer stepping a handful of sequences: launches and latency
+        dict(name="experts_tiny_4", op="experts", M=4, k=2, E=16, H=1024, I=512, shared=False, skew=0.0, pad=0),
+        # one user on a layer of 128 experts
+        dict(name="experts_1", op="experts", M=1, k=8, E=128, H=2048, I=768, shared=False, skew=0.0, pad=0),
+        # a server's decode step with a shared expert, 64 experts on this device; a captured batch with empty places
+        dict(name="experts_64_shared", op="experts", M=64, k=8, E=64, H=7168, I=2048, shared=True, skew=0.0, pad=5),
+        # a full prefill of the layer of 128 experts
+        dict(name="experts_8192", op="experts", M=8192, k=8, E=128, H=2048, I=768, shared=False, skew=0.0, pad=0),
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+MAX_FLOPS = 8192 * 8 * 6 * 2048 * 768
+MAX_WEIGHTS = 65 * 3 * 7168 * 2048  # values, the 64 experts and the shared one
+
+
+def draw(rng):
+    op = rng.choice(["linear", "grouped", "experts"])
+    c = dict(op=op)
+    if op == "linear":
+        c["N"] = _log_int(rng, 500, 7168) if rng.random() < 0.3 else 64 * _log_int(rng, 8, 112)
+        c["K"] = 16 * _log_int(rng, 32, 448)
+        c["M"] = max(1, min(_log_int(rng, 1, 8192), MAX_FLOPS // (2 * c["N"] * c["K"])))
+        c["out"] = rng.choice(["bf16", "bf16", "f32"])
+        return c
+    c["E"] = _log_int(rng, 16, 256)
+    c["k"] = rng.choice([2, 4, 6, 8, 8])
+    c["skew"] = rng.choice([0.0, 0.0, 0.7])
+    M = _log_int(rng, 1, 8192)
+    if op == "grouped":
+        c["fmt"] = rng.choice(["bf16", "int8"])
+        c["act"] = rng.random() < 0.5
+        c["weigh"] = not c["act"]
+        c["K"] = 16 * _log_int(rng, 32, 448)
+        c["N"] = 8 * _log_int(rng, 64, 256 if c["act"] else 896)
+        per = c["K"] * c["N"] * (2 if c["act"] else 1)
+        if rng.random() < 0.3:  # laid out by expert
+            c["k"] = 0
+        rows, pair = max(1, c["k"]), 2 if c["fmt"] == "bf16" else 1
+    else:
+        c["H"] = 64 * _log_int(rng, 16, 112)
+        c["I"] = 64 * _log_int(rng, 8, 32)
+        c["shared"] = rng.random() < 0.4
+        per = 3 * c["H"] * c["I"]
+        rows, pair = c["k"] + 1, 1
+    c["E"] = max(16, min(c["E"], MAX_WEIGHTS // (per * pair) - 1))
+    c["M"] = max(1, min(M, MAX_FLOPS // (rows * 2 * per)))
+    if op == "experts":
+        c["pad"] = rng.choice([0, 0, c["M"] // 9])
+    return c
+
+
+# ----------------------------------------------------------------------------- inputs
+
+
+def _int8_weights(shape, gen):
+    """Weights N(0, 0.02) with one scale per output channel of four deviations: codes and scales."""
+    q = torch.empty(shape, dtype=torch.bfloat16, device=DEV).normal_(0, 127 / 4, generator=gen)
+    s = torch.rand(shape[:-1], generator=gen, device=DEV).add_(0.5).mul_(0.02 * 4 / 127)
+    return q.round_().clamp_(-127, 127).to(torch.int8), s
+
+
+def _bf16_weights(shape, gen):
+    return torch.empty(shape, dtype=torch.bfloat16, device=DEV).normal_(0, 0.02, generator=gen)
+
+
+def _tokens(rows, width, gen):
+    """Normal activations with a few channels several times as large, as a residual stream has them."""
+    x = torch.randn((rows, width), generator=gen, device=DEV)
+    x[:, torch.randperm(width, generator=gen, device=DEV)[: max(1, width // 256)]] *= 6.0
+    return x.to(torch.bfloat16)
+
+
+def _routing(c, gen):
+    """Router weights and distinct expert ids of every token, [M, k]."""
+    logits = torch.randn((c["M"], c["E"]), generator=gen, device=DEV)
+    if c["skew"]:
+        p = (torch.randperm(c["E"], generator=gen, device=DEV).float() + 1) ** -c["skew"]
+        logits += torch.log(p / p.sum())
+    top = torch.topk(logits, c["k"], dim=1)
+    ids = top.indices.to(torch.int32)
+    if c.get("pad"):
+        ids[c["M"] - c["pad"] :] = -1  # the empty places of a captured batch
+    return torch.softmax(top.values, dim=1).contiguous(), ids.contiguous()
+
+
+def _shares(c, gen):
+    """Rows of every expert where the M rows come laid out by expert."""
+    p = torch.ones(c["E"], device=DEV)
+    if c["skew"]:
+        p = (torch.randperm(c["E"], generator=gen, device=DEV).float() + 1) ** -c["skew"]
+    owner = torch.multinomial(p, c["M"], replacement=True, generator=gen)
+    return torch.bincount(owner, minlength=c["E"])
+
+
+def prepare(case, seed):
+    c, gen = case, torch.Generator(device=DEV).manual_seed(int(seed))
+    s = {"case": c}
+    if c["op"] == "linear":
+        s["x"] = _tokens(c["M"], c["K"], gen)
+        s["w"], s["ws"] = _int8_weights((c["N"], c["K"]), gen)
+        return s
+    if c["op"] == "grouped":
+        s["x"] = _tokens(c["M"], c["K"], gen)
+        shape = (c["E"], c["N"] * (2 if c["act"] else 1), c["K"])
+        s["w"], s["ws"] = (_bf16_weights(shape, gen), None) if c["fmt"] == "bf16" else _int8_weights(shape, gen)
+        if c["k"] == 0:
+            counts = _shares(c, gen)
+            s["ids"], s["weights"] = None, torch.rand((c["M"],), generator=gen, device=DEV) if c["weigh"] else None
+            s["offsets"] = torch.cat([counts.new_zeros(1), counts.cumsum(0)]).to(torch.int32)
+            s["most"] = int(counts.max())  # what the plain form lays its rows out by
+            return s
+        weights, s["ids"] = _routing(c, gen)
+        s["weights"] = weights.view(-1) if c["weigh"] else None
+        s["most"] = int(torch.bincount(s["ids"].view(-1).long(), minlength=c["E"]).max())
+        return s
+    s["x"] = _tokens(c["M"], c["H"], gen)
+    s["tw"], s["ids"] = _routing(c, gen)
+    s["most"] = int(torch.bincount(s["ids"].view(-1).long().clamp_min(0), minlength=c["E"]).max())
+    s["bank"] = _int8_weights((c["E"], 2 * c["I"], c["H"]), gen) + _int8_weights((c["E"], c["H"], c["I"]), gen)
+    s["shared"] = None
+    if c["shared"]:
+        s["shared"] = _int8_weights((1, 2 * c["I"], c["H"]), gen) + _int8_weights((1, c["H"], c["I"]), gen)
+    return s
+
+
+# ----------------------------------------------------------------------------- the plain forms
+
+
+def _plain_quant(x):
+    """(codes as float32, scales) of every row; the quotient in 64 bits: its halves decide the codes."""
+    amax = x.float().abs().amax(-1, keepdim=True).double()
+    q = torch.where(amax > 0, x.double() * 127 / amax, 0.0).round()
+    return q.float(), (amax / 127).float()
+
+
+def _plain_products(x, w, owner, place, most):
+    """x[i] @ w[owner[i]].T in float32.  Few rows take their own copy of a matrix; many are laid out in a padded
+    batch, row i at place[i] of its owner's part."""
+    experts = w.shape[0]
+    if x.shape[0] <= experts:
+        return torch.bmm(w[owner].float(), x[:, :, None])[:, :, 0]
+    padded = x.new_zeros((experts, most, x.shape[1]))
+    padded[owner, place] = x
+    return torch.bmm(padded, w.float().transpose(1, 2))[owner, place]
+
+
+def _plain_groups(ids, experts):
+    """Order of the routes by expert, then each one's expert and place in its group; routes without one are left out."""
+    flat = ids.reshape(-1).long()
+    order = torch.sort(torch.where(flat < 0, experts, flat), stable=True).indices[: flat.shape[0]]
+    counts = torch.bincount(flat[flat >= 0], minlength=experts)
+    owner = torch.repeat_interleave(torch.arange(experts, device=DEV), counts)
+    starts = counts.cumsum(0) - counts
+    order = order[: owner.shape[0]]
+    return order, owner, torch.arange(owner.shape[0], device=DEV) - starts[owner]
+
+
+def _swiglu(h):
+    g, u = h.chunk(2, dim=-1)
+    return g / (1 + torch.exp(-g)) * u
+
+
+def _plain_grouped(c, s):
+    if s["ids"] is None:
+        counts = (s["offsets"][1:] - s["offsets"][:-1]).long()
+        owner = torch.repeat_interleave(torch.arange(c["E"], device=DEV), counts)
+        order = torch.arange(owner.shape[0], device=DEV)
+        place = order - s["offsets"].long()[owner]
+    else:
+        order, owner, place = _plain_groups(s["ids"], c["E"])
+    x, scale = (s["x"].float(), None) if c["fmt"] == "bf16" else _plain_quant(s["x"])
+    rows = order // max(1, c["k"])
+    h = _plain_products(x[rows], s["w"], owner, place, s["most"])
+    if scale is not None:
+        h = h * scale[rows] * s["ws"][owner]
+    if c["act"]:
+        h = _swiglu(h)
+    if s["weights"] is not None:
+        h = h * s["weights"][order][:, None]
+    y = torch.empty((order.shape[0], h.shape[1]), dtype=torch.bfloat16, device=DEV)
+    y[order] = h.to(torch.bfloat16)
+    return y
+
+
+def _plain_expert(x, scale, bank, owner, place, most):
+    """Both products of the rows x, their activations bf16 and then int8 in between; float32."""
+    gate_up, gs, down, ds = bank
+    h = _plain_products(x, gate_up, owner, place, most) * scale * gs[owner]
+    q, qs = _plain_quant(_swiglu(h).to(torch.bfloat16))
+    return _plain_products(q, down, owner, place, most) * qs * ds[owner]
+
+
+def _plain_experts(c, s):
+    q, scale = _plain_quant(s["x"])
+    order, owner, place = _plain_groups(s["ids"], c["E"])
+    rows = order // c["k"]
+    o = _plain_expert(q[rows], scale[rows], s["bank"], owner, place, s["most"])
+    routes = torch.zeros((c["M"] * c["k"], c["H"]), device=DEV)
+    routes[order] = o * s["tw"].view(-1)[order][:, None]
+    y = routes.view(c["M"], c["k"], c["H"]).sum(1)
+    if s["shared"] is not None:
+        every = torch.arange(c["M"], device=DEV)
+        y = y + _plain_expert(q, scale, s["shared"], torch.zeros_like(every), every, c["M"])
+    return y.to(torch.bfloat16)
+
+
+# ----------------------------------------------------------------------------- the calls
+
+
+_DTYPES = {"bf16": torch.bfloat16, "f32": torch.float32}
+
+
+def _own_run(c, s):
+    from freetoken_amd import ops
+
+    if c["op"] == "linear":
+        q, scale = ops.act_quant_int8(s["x"])
+        return ops.matmul_int8(q, scale, s["w"], s["ws"], out_dtype=_DTYPES[c["out"]])
+    if c["op"] == "grouped":
+        x, scale = s["x"], None
+        if c["fmt"] == "int8":
+            x, scale = ops.act_quant_int8(x)
+        act = "silu" if c["act"] else None
+        if s["ids"] is None:
+            return ops.grouped_matmul(x, s["w"], s["offsets"], x_scale=scale, w_scale=s["ws"], activation=act,
+                                      row_weight=s["weights"])
+        order, offsets = ops.group_routes(s["ids"], c["E"])
+        return ops.grouped_matmul(x, s["w"], offsets, order=order, top_k=c["k"], x_scale=scale, w_scale=s["ws"],
+                                  activation=act, row_weight=s["weights"])
+    gate_up, gs, down, ds = s["bank"]
+    bank = ops.ExpertBank("int8", gate_up, down, gs, ds)
+    shared = None
+    if s["shared"] is not None:
+        gate_up, gs, down, ds = s["shared"]
+        shared = ops.ExpertBank("int8", gate_up, down, gs, ds)
+    return ops.experts_int8(s["x"], s["tw"], s["ids"], bank, shared=shared)
+
+
+def run(state):
+    c, s = state["case"], state
+    if own:
+        return _own_run(c, s)
+    if c["op"] == "linear":
+        q, scale = _plain_quant(s["x"])
+        return (q @ s["w"].float().T * scale * s["ws"]).to(_DTYPES[c["out"]])
+    return _plain_grouped(c, s) if c["op"] == "grouped" else _plain_experts(c, s)
+
+
+# ----------------------------------------------------------------------------- what a pass needs
+
+
+def _touched(c):
+    """Experts that an even routing of the batch reaches."""
+    return c["E"] * (1.0 - (1.0 - max(1, c["k"]) / c["E"]) ** (c["M"] - c.get("pad", 0)))
+
+
+def work(case):
+    c, M = case, case["M"]
+    if c["op"] == "linear":
+        return {"bytes": c["N"] * (c["K"] + 4) + M * c["K"] * 2 + M * c["N"] * (2 if c["out"] == "bf16" else 4),
+                "flops": 2 * M * c["N"] * c["K"]}
+    rows = (M - c.get("pad", 0)) * max(1, c["k"])
+    if c["op"] == "grouped":
+        n = c["N"] * (2 if c["act"] else 1)
+        size = n * c["K"] * 2 if c["fmt"] == "bf16" else n * (c["K"] + 4)
+        return {"bytes": _touched(c) * size + M * c["K"] * 2 + rows * c["N"] * 2 + M * c["k"] * 4 * (1 + c["weigh"]),
+                "flops": 2 * rows * n * c["K"]}
+    size = 3 * c["H"] * c["I"] + 4 * (2 * c["I"] + c["H"])
+    more = 1 if c["shared"] else 0
+    return {"bytes": (_touched(c) + more) * size + M * c["H"] * 4 + M * c["k"] * 8,
+            "flops": (rows + more * M) * 6 * c["H"] * c["I"]}
+
+
+# ----------------------------------------------------------------------------- in 64 bits
+
+
+def _exact_codes(x):
+    """The values that the codes of the rows of x stand for."""
+    x = x.double()
+    a = x.abs().amax(dim=-1, keepdim=True)
+    a = torch.where(a > 0, a, 1.0)
+    return torch.round((127 * x) / a) * (a / 127)
+
+
+def _exact_matrix(w, s):
+    return w.double() if s is None else w.double() * s.double()[..., None]
+
+
+def _exact_act(h):
+    g, u = h[:, : h.shape[1] // 2], h[:, h.shape[1] // 2 :]
+    return g * torch.sigmoid(g) * u
+
+
+def exact(case, seed):
+    c, s = case, prepare(case, seed)
+    x = _exact_codes(s["x"]) if c.get("fmt") != "bf16" else s["x"].double()
+    if c["op"] == "linear":
+        return x @ _exact_matrix(s["w"], s["ws"]).T
+    if c["op"] == "grouped":
+        flat = None if s["ids"] is None else s["ids"].view(-1)
+        y = torch.zeros((c["M"] * max(1, c["k"]), c["N"]), dtype=torch.float64, device=DEV)
+        for e in range(c["E"]):
+            if flat is None:
+                at = torch.arange(int(s["offsets"][e]), int(s["offsets"][e + 1]), device=DEV)
+            else:
+                at = torch.nonzero(flat == e)[:, 0]
+            if at.numel():
+                h = x[at // max(1, c["k"])] @ _exact_matrix(s["w"][e], None if s["ws"] is None else s["ws"][e]).T
+                y[at] = _exact_act(h) if c["act"] else h
+        return y if s["weights"] is None else y * s["weights"].double()[:, None]
+
+    def mlp(rows, bank, e):
+        a = _exact_act(rows @ _exact_matrix(bank[0][e], bank[1][e]).T)
+        return _exact_codes(a.to(torch.bfloat16)) @ _exact_matrix(bank[2][e], bank[3][e]).T
+
+    y = torch.zeros((c["M"], c["H"]), dtype=torch.float64, device=DEV)
+    for e in range(c["E"]):
+        token, place = torch.nonzero(s["ids"] == e, as_tuple=True)
+        if token.numel():
+            y.index_add_(0, token, mlp(x[token], s["bank"], e) * s["tw"].double()[token, place][:, None])
+    return y if s["shared"] is None else y + mlp(x, s["shared"], 0)
