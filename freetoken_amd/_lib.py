@@ -20,7 +20,8 @@ FTMOE_ERR_BUSY = -5
 FTMOE_ERR_TIMEOUT = -6
 
 DTYPE_F32, DTYPE_BF16 = 0, 1
-FMT_NONE, FMT_BF16, FMT_FP8_B128, FMT_MXFP4 = -1, 0, 1, 2
+FMT_NONE, FMT_BF16, FMT_FP8_B128, FMT_MXFP4, FMT_INT8 = -1, 0, 1, 2, 3
+ACT_NONE = -1
 ACT = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
 
 # Every symbol include/ftmoe.h declares, with (restype, argtypes).
@@ -72,6 +73,27 @@ class FtmoeFetchBank(ctypes.Structure):
 
 _fbp = ctypes.POINTER(FtmoeFetchBank)
 
+
+class FtmoeGrouped(ctypes.Structure):
+    _fields_ = [
+        ("format", ctypes.c_int),
+        ("num_experts", ctypes.c_int),
+        ("N", ctypes.c_int),
+        ("K", ctypes.c_int),
+        ("x", ctypes.c_void_p),
+        ("x_scale", ctypes.c_void_p),
+        ("w", ctypes.c_void_p),
+        ("w_scale", ctypes.c_void_p),
+        ("x_rows", ctypes.c_int),
+        ("top_k", ctypes.c_int),
+        ("offsets", ctypes.c_void_p),
+        ("order", ctypes.c_void_p),
+        ("row_weight", ctypes.c_void_p),
+        ("activation", ctypes.c_int),
+        ("y", ctypes.c_void_p),
+    ]
+
+
 SIGNATURES = {
     "ftmoe_last_error": (ctypes.c_char_p, []),
     "ftmoe_version": (_i, []),
@@ -100,6 +122,13 @@ SIGNATURES = {
                                          _bp, _bp, _i, _i, _vp, _vp, _sz, _vp]),
     "ftmoe_experts_prefill_workspace": (_sz, [_i, _i, _bp, _bp]),
     "ftmoe_experts_prefill": (_i, [_vp, _i, _i, _vp, _vp, _bp, _bp, _i, _vp, _vp, _sz, _vp]),
+    "ftmoe_act_quant_int8": (_i, [_vp, _i, _i, _vp, _vp, _vp]),
+    "ftmoe_matmul_int8": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp]),
+    "ftmoe_group_routes_workspace": (_sz, [_i, _i]),
+    "ftmoe_group_routes": (_i, [_vp, _i, _i, _vp, _vp, _vp, _sz, _vp]),
+    "ftmoe_grouped_matmul": (_i, [ctypes.POINTER(FtmoeGrouped), _vp]),
+    "ftmoe_experts_int8_workspace": (_sz, [_i, _i, _bp, _bp]),
+    "ftmoe_experts_int8": (_i, [_vp, _i, _i, _vp, _vp, _bp, _bp, _i, _vp, _vp, _sz, _vp]),
     "ftmoe_cpu_executor_create": (_vp, [_i]),
     "ftmoe_cpu_executor_destroy": (_i, [_vp, _i]),
     "ftmoe_cpu_executor_healthy": (_i, [_vp]),

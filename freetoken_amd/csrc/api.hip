@@ -797,6 +797,337 @@ int ftmoe_experts_prefill(const void* x, int M, int top_k, const float* topk_w, 
 
 }  // extern "C"
 
+// ---- 8-bit integers and ragged groups ----------------------------------------
+namespace {
+
+constexpr int kInt8MaxK = 131056;  // 127 * 128 * K stays below 2^31
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+int check_product(const ftmoe::MatmulArgs& a, const char* what) {
+  const int step = a.int8 ? 16 : 8, most = a.int8 ? kInt8MaxK : INT32_MAX / 4;
+  if (a.N <= 0 || a.K <= 0 || a.K % step || a.K > most)
+    return fail(FTMOE_ERR_UNSUPPORTED, "%s: N=%d K=%d (K a positive multiple of %d, at most %d)", what, a.N, a.K, step,
+                most);
+  if (a.act < FTMOE_ACT_NONE || a.act > FTMOE_ACT_GELU_TANH)
+    return fail(FTMOE_ERR_UNSUPPORTED, "%s: activation %d", what, a.act);
+  if (a.act != FTMOE_ACT_NONE && a.N % 2)
+    return fail(FTMOE_ERR_INVALID, "%s: N=%d holds no gate and up halves", what, a.N);
+  const size_t row = static_cast<size_t>(a.K) * (a.int8 ? 1 : 2), lim = size_t{1} << 31;
+  if (row * a.x_rows >= lim || row * 256 >= lim)
+    return fail(FTMOE_ERR_UNSUPPORTED, "%s: x of %d rows or 256 rows of w of K=%d reach 2 GiB", what, a.x_rows, a.K);
+  if (a.rows == 0) return FTMOE_OK;
+  if (!a.x || !a.w || !a.y || (a.int8 && (!a.xs || !a.ws))) return fail(FTMOE_ERR_INVALID, "%s: NULL pointer", what);
+  if (!aligned16(a.x) || !aligned16(a.w) || !aligned16(a.y))
+    return fail(FTMOE_ERR_UNSUPPORTED, "%s: x, w and y must be 16-byte aligned", what);
+  return FTMOE_OK;
+}
+
+// A bank of the int8 expert layer.
+int check_int8_bank(const ftmoe_bank* b, const char* name, bool shared) {
+  if (!b) return fail(FTMOE_ERR_INVALID, "%s bank is NULL", name);
+  if (b->format != FTMOE_FMT_INT8)
+    return fail(FTMOE_ERR_UNSUPPORTED, "experts_int8: %s bank of format %d", name, b->format);
+  if (b->hidden <= 0 || b->inter <= 0 || b->hidden % 16 || b->inter % 16 || b->hidden > kInt8MaxK ||
+      b->inter > kInt8MaxK)
+    return fail(FTMOE_ERR_UNSUPPORTED, "%s bank: hidden %d / inter %d must be positive multiples of 16, at most %d", name,
+                b->hidden, b->inter, kInt8MaxK);
+  if (b->num_rows <= 0 || (shared && b->num_rows != 1))
+    return fail(FTMOE_ERR_INVALID, "%s bank: num_rows %d", name, b->num_rows);
+  if (b->num_rows > ftmoe::kCountMaxRows)
+    return fail(FTMOE_ERR_UNSUPPORTED, "experts_int8: num_rows %d > %d", b->num_rows, ftmoe::kCountMaxRows);
+  if (!b->gate_up || !b->down || !b->gate_up_scale || !b->down_scale)
+    return fail(FTMOE_ERR_INVALID, "%s bank: NULL weights or scales", name);
+  if (!std::isfinite(b->swiglu_limit) || b->swiglu_limit < 0.f)
+    return fail(FTMOE_ERR_INVALID, "%s bank: swiglu_limit %g (finite, >= 0)", name, b->swiglu_limit);
+  return FTMOE_OK;
+}
+
+// Routes up to which one workgroup groups them; more are counted by several.
+constexpr int kGroupOneWorkgroup = 4096;
+
+struct GroupLayout {
+  int32_t* total;
+  int32_t* gcount;
+  size_t bytes;
+};
+
+GroupLayout group_layout(void* ws, int numel, int num_experts) {
+  GroupLayout L{};
+  Carver c{static_cast<uint8_t*>(ws)};
+  L.total = c.take<int32_t>(1);
+  L.gcount = c.take<int32_t>(ftmoe::align_gcount_ints(numel, num_experts));
+  L.bytes = c.off;
+  return L;
+}
+
+hipError_t launch_group_routes(const int32_t* ids, int numel, int num_experts, int32_t* order, int32_t* offsets,
+                               const GroupLayout& L, ftmoe_stream_t stream) {
+  ftmoe::AlignArgs a{};
+  a.ids = ids;
+  a.numel = numel;
+  a.num_experts = num_experts;
+  a.block_size = 1;
+  a.sorted_ids = order;
+  a.max_padded = numel;
+  a.ntpp = L.total;
+  a.cum_out = offsets;
+  return numel <= kGroupOneWorkgroup ? ftmoe::launch_align(a, stream) : ftmoe::launch_align_large(a, L.gcount, stream);
+}
+
+struct Int8Layout {
+  int32_t* order;
+  int32_t* offsets;
+  GroupLayout group;
+  int8_t* xq;
+  float* xs;
+  uint16_t* act;    // [routes, inter], then the shared expert's [M, inter]
+  int8_t* actq;
+  float* as;
+  uint16_t* routes;  // [routes, hidden]
+  uint16_t* sh_act;
+  int8_t* sh_actq;
+  float* sh_as;
+  float* sh_out;     // [M, hidden]
+  size_t bytes;
+};
+
+Int8Layout int8_layout(void* ws, int M, int k, const ftmoe_bank* bank, const ftmoe_bank* shared) {
+  Int8Layout L{};
+  Carver c{static_cast<uint8_t*>(ws)};
+  const int numel = M * k;
+  const size_t H = bank->hidden, I = bank->inter;
+  L.order = c.take<int32_t>(numel);
+  L.offsets = c.take<int32_t>(bank->num_rows + 2);
+  L.group = group_layout(ws ? static_cast<uint8_t*>(ws) + c.off : nullptr, numel, bank->num_rows);
+  c.off += L.group.bytes;
+  L.xq = c.take<int8_t>(M * H);
+  L.xs = c.take<float>(M);
+  L.act = c.take<uint16_t>(numel * I);
+  L.actq = c.take<int8_t>(numel * I);
+  L.as = c.take<float>(numel);
+  L.routes = c.take<uint16_t>(numel * H);
+  if (shared) {
+    const size_t Is = shared->inter;
+    L.sh_act = c.take<uint16_t>(M * Is);
+    L.sh_actq = c.take<int8_t>(M * Is);
+    L.sh_as = c.take<float>(M);
+    L.sh_out = c.take<float>(M * H);
+  }
+  L.bytes = c.off;
+  return L;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ftmoe_act_quant_int8(const void* x, int rows, int K, void* q, float* scales, ftmoe_stream_t stream) {
+  if (rows < 0) return fail(FTMOE_ERR_INVALID, "act_quant_int8: rows=%d", rows);
+  if (K <= 0 || K % 16) return fail(FTMOE_ERR_UNSUPPORTED, "act_quant_int8: K=%d (a positive multiple of 16)", K);
+  if (rows == 0) return FTMOE_OK;
+  if (!x || !q || !scales) return fail(FTMOE_ERR_INVALID, "act_quant_int8: NULL pointer");
+  if (!aligned16(x) || !aligned16(q))
+    return fail(FTMOE_ERR_UNSUPPORTED, "act_quant_int8: x and q must be 16-byte aligned");
+  return check_hip(ftmoe::launch_act_quant_int8(static_cast<const uint16_t*>(x), rows, K, static_cast<int8_t*>(q),
+                                                scales, stream),
+                   "act_quant_int8 launch");
+}
+
+int ftmoe_matmul_int8(const void* q, const float* q_scale, const void* w, const float* w_scale, int M, int N, int K,
+                      int activation, int out_dtype, void* y, ftmoe_stream_t stream) {
+  if (M < 0) return fail(FTMOE_ERR_INVALID, "matmul_int8: M=%d", M);
+  if (out_dtype != FTMOE_DTYPE_BF16 && out_dtype != FTMOE_DTYPE_F32)
+    return fail(FTMOE_ERR_UNSUPPORTED, "matmul_int8: output dtype %d", out_dtype);
+  ftmoe::MatmulArgs a{};
+  a.int8 = 1;
+  a.x = static_cast<const uint8_t*>(q);
+  a.xs = q_scale;
+  a.w = static_cast<const uint8_t*>(w);
+  a.ws = w_scale;
+  a.E = 1;
+  a.N = N;
+  a.K = K;
+  a.rows = a.x_rows = M;
+  a.top_k = 1;
+  a.act = activation;
+  a.out_f32 = out_dtype == FTMOE_DTYPE_F32;
+  a.y = y;
+  const int rc = check_product(a, "matmul_int8");
+  if (rc || M == 0) return rc;
+  return check_hip(ftmoe::launch_matmul(a, stream), "matmul_int8 launch");
+}
+
+size_t ftmoe_group_routes_workspace(int numel, int num_experts) {
+  if (numel < 0 || num_experts <= 0) return 0;
+  return group_layout(nullptr, numel, num_experts).bytes;
+}
+
+int ftmoe_group_routes(const int32_t* topk_ids, int numel, int num_experts, int32_t* order, int32_t* offsets,
+                       void* workspace, size_t workspace_bytes, ftmoe_stream_t stream) {
+  if (numel < 0) return fail(FTMOE_ERR_INVALID, "group_routes: numel=%d", numel);
+  if (num_experts <= 0 || num_experts > ftmoe::kCountMaxRows)
+    return fail(FTMOE_ERR_UNSUPPORTED, "group_routes: num_experts=%d (1 to %d)", num_experts, ftmoe::kCountMaxRows);
+  if (((!topk_ids || !order) && numel) || !offsets) return fail(FTMOE_ERR_INVALID, "group_routes: NULL pointer");
+  const size_t need = group_layout(nullptr, numel, num_experts).bytes;
+  if (!workspace || workspace_bytes < need)
+    return fail(FTMOE_ERR_WORKSPACE, "group_routes: workspace %zu < %zu bytes", workspace_bytes, need);
+  return check_hip(launch_group_routes(topk_ids, numel, num_experts, order, offsets,
+                                       group_layout(workspace, numel, num_experts), stream),
+                   "group_routes launch");
+}
+
+int ftmoe_grouped_matmul(const ftmoe_grouped* g, ftmoe_stream_t stream) {
+  if (!g) return fail(FTMOE_ERR_INVALID, "grouped_matmul: NULL arguments");
+  if (g->format != FTMOE_FMT_BF16 && g->format != FTMOE_FMT_INT8)
+    return fail(FTMOE_ERR_UNSUPPORTED, "grouped_matmul: format %d (bf16 or int8)", g->format);
+  if (g->x_rows < 0 || g->top_k <= 0 || (!g->order && g->top_k != 1) ||
+      static_cast<long long>(g->x_rows) * g->top_k > INT32_MAX)
+    return fail(FTMOE_ERR_INVALID, "grouped_matmul: x_rows=%d top_k=%d (1 without an order)", g->x_rows, g->top_k);
+  if (g->num_experts <= 0 || g->num_experts > ftmoe::kCountMaxRows)
+    return fail(FTMOE_ERR_UNSUPPORTED, "grouped_matmul: num_experts=%d (1 to %d)", g->num_experts, ftmoe::kCountMaxRows);
+  ftmoe::MatmulArgs a{};
+  a.int8 = g->format == FTMOE_FMT_INT8;
+  a.x = static_cast<const uint8_t*>(g->x);
+  a.xs = g->x_scale;
+  a.w = static_cast<const uint8_t*>(g->w);
+  a.ws = g->w_scale;
+  a.E = g->num_experts;
+  a.N = g->N;
+  a.K = g->K;
+  a.x_rows = g->x_rows;
+  a.rows = g->x_rows * g->top_k;
+  a.offsets = g->offsets;
+  a.order = g->order;
+  a.top_k = g->top_k;
+  a.row_weight = g->row_weight;
+  a.act = g->activation;
+  a.y = g->y;
+  const int rc = check_product(a, "grouped_matmul");
+  if (rc || a.rows == 0) return rc;
+  if (!a.offsets) return fail(FTMOE_ERR_INVALID, "grouped_matmul: NULL offsets");
+  return check_hip(ftmoe::launch_matmul(a, stream), "grouped_matmul launch");
+}
+
+size_t ftmoe_experts_int8_workspace(int M, int top_k, const ftmoe_bank* bank, const ftmoe_bank* shared) {
+  if (!bank || M <= 0 || top_k <= 0) return 0;
+  return int8_layout(nullptr, M, top_k, bank, shared).bytes;
+}
+
+int ftmoe_experts_int8(const void* x, int M, int top_k, const float* topk_w, const int32_t* topk_ids,
+                       const ftmoe_bank* bank, const ftmoe_bank* shared, int activation, void* y, void* workspace,
+                       size_t workspace_bytes, ftmoe_stream_t stream) {
+  int rc = check_int8_bank(bank, "routed", false);
+  if (rc) return rc;
+  if (shared) {
+    rc = check_int8_bank(shared, "shared", true);
+    if (rc) return rc;
+    if (shared->hidden != bank->hidden)
+      return fail(FTMOE_ERR_INVALID, "shared hidden %d != %d", shared->hidden, bank->hidden);
+  }
+  if (M < 0 || top_k <= 0 || static_cast<long long>(M) * top_k > INT32_MAX)
+    return fail(FTMOE_ERR_INVALID, "experts_int8: M=%d top_k=%d", M, top_k);
+  if (activation < FTMOE_ACT_SILU || activation > FTMOE_ACT_GELU_TANH)
+    return fail(FTMOE_ERR_UNSUPPORTED, "experts_int8: activation %d", activation);
+  rc = check_limit(bank, shared, activation, "experts_int8");
+  if (rc) return rc;
+  if (M == 0) return FTMOE_OK;
+  if (!x || !topk_w || !topk_ids || !y) return fail(FTMOE_ERR_INVALID, "experts_int8: NULL pointer");
+  if (!aligned16(x) || !aligned16(y)) return fail(FTMOE_ERR_UNSUPPORTED, "experts_int8: x and y must be 16-byte aligned");
+  const size_t need = int8_layout(nullptr, M, top_k, bank, shared).bytes;
+  if (!workspace || workspace_bytes < need)
+    return fail(FTMOE_ERR_WORKSPACE, "experts_int8: workspace %zu < %zu bytes", workspace_bytes, need);
+  const Int8Layout L = int8_layout(workspace, M, top_k, bank, shared);
+  const int numel = M * top_k, H = bank->hidden;
+
+  // the two products of one bank's rows
+  ftmoe::MatmulArgs up{}, down{};
+  up.int8 = down.int8 = 1;
+  up.x = reinterpret_cast<const uint8_t*>(L.xq);
+  up.xs = L.xs;
+  up.w = static_cast<const uint8_t*>(bank->gate_up);
+  up.ws = static_cast<const float*>(bank->gate_up_scale);
+  up.E = down.E = bank->num_rows;
+  up.N = 2 * bank->inter;
+  up.K = H;
+  up.x_rows = M;
+  up.rows = numel;
+  up.offsets = down.offsets = L.offsets;
+  up.order = down.order = L.order;
+  up.top_k = top_k;
+  up.act = activation;
+  up.limit = bank->swiglu_limit;
+  up.y = L.act;
+  down.x = reinterpret_cast<const uint8_t*>(L.actq);
+  down.xs = L.as;
+  down.w = static_cast<const uint8_t*>(bank->down);
+  down.ws = static_cast<const float*>(bank->down_scale);
+  down.N = H;
+  down.K = bank->inter;
+  down.x_rows = down.rows = numel;
+  down.top_k = 1;
+  down.act = FTMOE_ACT_NONE;
+  down.row_weight = topk_w;
+  down.y = L.routes;
+  for (const ftmoe::MatmulArgs* a : {&up, &down}) {
+    rc = check_product(*a, "experts_int8");
+    if (rc) return rc;
+  }
+  ftmoe::MatmulArgs sh_up = up, sh_down = down;
+  if (shared) {
+    sh_up.w = static_cast<const uint8_t*>(shared->gate_up);
+    sh_up.ws = static_cast<const float*>(shared->gate_up_scale);
+    sh_up.E = sh_down.E = 1;
+    sh_up.N = 2 * shared->inter;
+    sh_up.offsets = sh_down.offsets = nullptr;
+    sh_up.order = sh_down.order = nullptr;
+    sh_up.rows = sh_down.rows = sh_down.x_rows = M;
+    sh_up.top_k = 1;
+    sh_up.limit = shared->swiglu_limit;
+    sh_up.y = L.sh_act;
+    sh_down.x = reinterpret_cast<const uint8_t*>(L.sh_actq);
+    sh_down.xs = L.sh_as;
+    sh_down.w = static_cast<const uint8_t*>(shared->down);
+    sh_down.ws = static_cast<const float*>(shared->down_scale);
+    sh_down.K = shared->inter;
+    sh_down.row_weight = nullptr;
+    sh_down.out_f32 = 1;
+    sh_down.y = L.sh_out;
+    for (const ftmoe::MatmulArgs* a : {&sh_up, &sh_down}) {
+      rc = check_product(*a, "experts_int8");
+      if (rc) return rc;
+    }
+  }
+
+  const auto run = [&](hipError_t err, const char* what) {
+    if (rc == FTMOE_OK) rc = check_hip(err, what);
+    return rc == FTMOE_OK;
+  };
+  if (!run(launch_group_routes(topk_ids, numel, bank->num_rows, L.order, L.offsets, L.group, stream),
+           "experts_int8 grouping"))
+    return rc;
+  if (!run(ftmoe::launch_act_quant_int8(static_cast<const uint16_t*>(x), M, H, L.xq, L.xs, stream), "experts_int8 x quant"))
+    return rc;
+  if (!run(ftmoe::launch_matmul(up, stream), "experts_int8 gate_up")) return rc;
+  // (rows of skipped routes hold what the workspace held: quantised, never multiplied)
+  if (!run(ftmoe::launch_act_quant_int8(L.act, numel, bank->inter, L.actq, L.as, stream), "experts_int8 act quant"))
+    return rc;
+  if (!run(ftmoe::launch_matmul(down, stream), "experts_int8 down")) return rc;
+  if (shared) {
+    if (!run(ftmoe::launch_matmul(sh_up, stream), "experts_int8 shared gate_up")) return rc;
+    if (!run(ftmoe::launch_act_quant_int8(L.sh_act, M, shared->inter, L.sh_actq, L.sh_as, stream),
+             "experts_int8 shared act quant"))
+      return rc;
+    if (!run(ftmoe::launch_matmul(sh_down, stream), "experts_int8 shared down")) return rc;
+  }
+  run(ftmoe::launch_combine_routes(L.routes, topk_ids, bank->num_rows, L.sh_out, M, top_k, H,
+                                   static_cast<uint16_t*>(y), stream),
+      "experts_int8 combine");
+  return rc;
+}
+
+}  // extern "C"
+
 // ---- decode without allocation ---------------------------------------------
 // The workspace of ftmoe_experts_decode_noalloc is this file-scope device
 // array: each GPU the library runs on holds its own copy for the life of the

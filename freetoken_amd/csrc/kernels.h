@@ -7,7 +7,7 @@
 
 namespace ftmoe {
 
-enum WFmt : int { FMT_BF16 = 0, FMT_FP8 = 1, FMT_MXFP4 = 2, FMT_NONE = -1 };
+enum WFmt : int { FMT_BF16 = 0, FMT_FP8 = 1, FMT_MXFP4 = 2, FMT_INT8 = 3, FMT_NONE = -1 };
 
 struct AlignArgs {
   const int32_t* ids;          // [numel] expert ids (or expert ids to map)
@@ -273,6 +273,34 @@ int fetch_chunks(uint64_t row_bytes);
 
 // Records the message of a failed C-ABI call (ftmoe_last_error) and returns code.
 int report_error(int code, const char* msg);
+
+// Matrix products with one weight matrix per group of rows (matmul.hip):
+//   y[r] = g[r] * act(x[r / top_k] . w[e]^T)  for r = order[i], offsets[e] <= i < offsets[e + 1]
+// (order null: r = i; offsets null: one group of all rows).
+struct MatmulArgs {
+  int int8;                 // 1: x, w int8 with xs, ws; 0: bf16
+  const uint8_t* x;         // [x_rows, K]
+  const float* xs;          // int8: [x_rows] scale of every row of x
+  const uint8_t* w;         // [E, N, K]; with act: gate rows [0, N/2), up rows [N/2, N) of every matrix
+  const float* ws;          // int8: [E, N] scale of every output channel
+  int E, N, K;
+  int rows, x_rows;         // rows of y (= top_k * x_rows) and of x
+  const int32_t* offsets;   // nullable [E + 1]
+  const int32_t* order;     // nullable [rows]
+  int top_k;
+  const float* row_weight;  // nullable [rows]
+  int act;                  // -1: none, else Act
+  float limit;              // clamped SwiGLU (> 0), else 0
+  int out_f32;              // y float32 instead of bf16
+  void* y;                  // [rows, N] ([rows, N/2] with act)
+};
+hipError_t launch_matmul(const MatmulArgs& a, hipStream_t stream);
+hipError_t launch_act_quant_int8(const uint16_t* x, int rows, int K, int8_t* q, float* scales, hipStream_t stream);
+// The routes' rows of every token (ids outside [0, num_rows) skipped) and its float32 shared row (nullable), summed
+// in float32 and rounded once.
+hipError_t launch_combine_routes(const uint16_t* routes, const int32_t* ids, int num_rows, const float* shared, int M,
+                                 int k, int H, uint16_t* y, hipStream_t stream);
+
 hipError_t launch_combine(const uint16_t* ic3, const int32_t* ids, int num_rows, const uint16_t* sh_out, int M,
                           int k, int H, uint16_t* y, hipStream_t stream);
 

@@ -3,7 +3,10 @@ the gfx950 kernels: drop-in for ``MoELayer``, ``OffloadMoELayer`` and
 ``make_moe_layer``.
 
 Differences from the reference, all additive:
-  * ``weight_format`` also accepts ``"ds_fp4"`` (row-major MXFP4 resident banks);
+  * ``weight_format`` also accepts ``"ds_fp4"`` (row-major MXFP4 resident banks)
+    and ``"int8"`` (W8A8 resident banks: int8 ``gate_up_proj`` and ``down_proj``
+    with one float32 scale per output channel, ``gate_up_scale`` and
+    ``down_scale``; ``ops.quantize_bank_int8`` makes them from bf16);
   * an optional ``shared_expert`` (``ops.ExpertBank`` with one row) is added to
     the routed output inside the expert kernels, replacing the model block's
     separate ``out + shared_experts(x)`` (``models/glm4_moe/moe.py:81-82``);
@@ -89,6 +92,12 @@ class MoELayer:
             self.down_proj = torch.empty(n, h, inter // 2, dtype=torch.uint8, device=dev)
             self.down_scale = torch.empty(n, h, inter // 32, dtype=torch.uint8, device=dev)
             return
+        if self.weight_format == "int8":
+            self.gate_up_proj = torch.empty(n, 2 * inter, h, dtype=torch.int8, device=dev)
+            self.gate_up_scale = torch.empty(n, 2 * inter, dtype=torch.float32, device=dev)
+            self.down_proj = torch.empty(n, h, inter, dtype=torch.int8, device=dev)
+            self.down_scale = torch.empty(n, h, dtype=torch.float32, device=dev)
+            return
         assert self.weight_format == "bf16", f"no resident expert allocation for weight_format {self.weight_format!r}"
         self.gate_up_proj = torch.empty(n, 2 * inter, h, dtype=torch.bfloat16, device=dev)
         self.down_proj = torch.empty(n, h, inter, dtype=torch.bfloat16, device=dev)
@@ -99,6 +108,9 @@ class MoELayer:
                                   self.down_scale_inv)
         if self.weight_format == "ds_fp4":
             return ops.ExpertBank("mxfp4", self.gate_up_proj, self.down_proj, self.gate_up_scale, self.down_scale,
+                                  swiglu_limit=float(self.swiglu_limit or 0.0))
+        if self.weight_format == "int8":
+            return ops.ExpertBank("int8", self.gate_up_proj, self.down_proj, self.gate_up_scale, self.down_scale,
                                   swiglu_limit=float(self.swiglu_limit or 0.0))
         return ops.ExpertBank("bf16", self.gate_up_proj, self.down_proj)
 
@@ -119,6 +131,9 @@ class MoELayer:
                                       activation=self.activation,
                                       apply_router_weight_on_input=self.apply_router_weight_on_input)
         assert not self.apply_router_weight_on_input or self.weight_format == "bf16"
+        if self.weight_format == "int8":  # one path for both phases
+            return ops.experts_int8(hidden_states, topk_weights, topk_ids, self.bank(), shared=self.shared_expert,
+                                    activation=self.activation)
         fn = ops.experts_prefill if prefill else ops.experts_decode
         return fn(hidden_states, topk_weights, topk_ids, self.bank(), shared=self.shared_expert,
                   activation=self.activation)
@@ -139,7 +154,8 @@ class MoELayer:
                 activation=self.activation, apply_router_weight_on_input=self.apply_router_weight_on_input,
             )
             return self._maybe_all_reduce(out)
-        if not _is_prefill(hidden_states.shape[0] * self.top_k) and router_logits is not None:
+        if self.weight_format != "int8" and not _is_prefill(hidden_states.shape[0] * self.top_k) \
+                and router_logits is not None:
             # decode: router and experts in one call (router + permutation in one
             # launch for small batches)
             assert not self.apply_router_weight_on_input or self.weight_format == "bf16"

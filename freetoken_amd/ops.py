@@ -292,9 +292,145 @@ def act_quant_fp8(x: torch.Tensor, mode: int = 0):
     return q, s
 
 
+# --------------------------------------------------------------------------- 8-bit integers, ragged groups
+
+
+def _one_device(*tensors: torch.Tensor | None) -> torch.device:
+    """The device that holds all the tensors."""
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) != 1:
+        raise ValueError(f"tensors on different devices: {sorted(map(str, devices))}")
+    return devices.pop()
+
+
+def _act_code(activation: str | None) -> int:
+    if activation is None:
+        return _lib.ACT_NONE
+    if activation not in _lib.ACT:
+        raise ValueError(f"Unsupported activation: {activation}")
+    return _lib.ACT[activation]
+
+
+def act_quant_int8(x: torch.Tensor):
+    """Symmetric 8-bit quantisation of bf16 rows (last dimension; a multiple of
+    16): returns (codes int8 shaped like ``x``, scales float32 of its leading
+    dimensions), ``x`` being about ``codes * scale``.  The rows are tokens, or a
+    weight matrix's output channels (see ftmoe_act_quant_int8)."""
+    if x.dtype != torch.bfloat16:
+        raise ValueError("x must be bfloat16")
+    if x.dim() < 1:
+        raise ValueError("x must have rows")
+    _require_gpu(x)
+    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    s = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    with torch.cuda.device(x.device):
+        check(lib().ftmoe_act_quant_int8(_ptr(x), s.numel(), x.shape[-1], _ptr(q), _ptr(s), _stream(x.device)),
+              "act_quant_int8")
+    return q, s
+
+
+def matmul_int8(q: torch.Tensor, q_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+                activation: str | None = None, out: torch.Tensor | None = None,
+                out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``(q @ w.T) * q_scale[:, None] * w_scale`` with exact integer sums: ``q``
+    int8 [M, K] and ``q_scale`` float32 [M] (``act_quant_int8``), ``w`` int8 [N, K]
+    and ``w_scale`` float32 [N]; K a multiple of 16.  With an ``activation`` the
+    first N/2 rows of ``w`` are gate and the others up rows, and the result [M,
+    N/2] is ``act(gate) * up``.  ``out_dtype`` (or ``out``'s) is bfloat16 or float32."""
+    if q.dtype != torch.int8 or w.dtype != torch.int8 or q.dim() != 2 or w.dim() != 2 or q.shape[1] != w.shape[1]:
+        raise ValueError("q and w must be int8 [M, K] and [N, K]")
+    if q_scale.dtype != torch.float32 or w_scale.dtype != torch.float32:
+        raise ValueError("scales must be float32")
+    if q_scale.shape != q.shape[:1] or w_scale.shape != w.shape[:1]:
+        raise ValueError("one scale per row of q and of w")
+    act = _act_code(activation)
+    _require_gpu(q, q_scale, w, w_scale, out)
+    (m, k), n = q.shape, w.shape[0]
+    dev = _one_device(q, q_scale, w, w_scale, out)
+    shape = (m, n if activation is None else n // 2)
+    y = out if out is not None else torch.empty(shape, dtype=out_dtype, device=dev)
+    if y.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("the result is bfloat16 or float32")
+    if tuple(y.shape) != shape:
+        raise ValueError(f"out must be {shape}")
+    with torch.cuda.device(dev):
+        check(lib().ftmoe_matmul_int8(_ptr(q), _ptr(q_scale), _ptr(w), _ptr(w_scale), m, n, k, act,
+                                      _lib.DTYPE_F32 if y.dtype == torch.float32 else _lib.DTYPE_BF16, _ptr(y),
+                                      _stream(dev)), "matmul_int8")
+    return y
+
+
+def group_routes(topk_ids: torch.Tensor, num_experts: int):
+    """Routes by expert (stable, as ``align`` with block size 1): returns (order
+    int32 [numel], the flat route indices of expert 0, 1, ...; offsets int32
+    [num_experts + 1], expert e's positions being offsets[e] to offsets[e + 1]).
+    Ids outside [0, num_experts) belong to no expert: their routes are not
+    among those positions."""
+    if topk_ids.dtype != torch.int32:
+        raise ValueError("topk_ids must be int32")
+    _require_gpu(topk_ids)
+    dev, numel = topk_ids.device, topk_ids.numel()
+    order = torch.empty((numel,), dtype=torch.int32, device=dev)
+    offsets = torch.empty((max(num_experts, 0) + 2,), dtype=torch.int32, device=dev)
+    ws = torch.empty((lib().ftmoe_group_routes_workspace(numel, num_experts),), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        check(lib().ftmoe_group_routes(_ptr(topk_ids), numel, num_experts, _ptr(order), _ptr(offsets), _ptr(ws),
+                                       ws.numel(), _stream(dev)), "group_routes")
+    return order, offsets[: num_experts + 1]
+
+
+def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, order: torch.Tensor | None = None,
+                   top_k: int = 1, x_scale: torch.Tensor | None = None, w_scale: torch.Tensor | None = None,
+                   row_weight: torch.Tensor | None = None, activation: str | None = None,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """Matrix products grouped by expert, each with a ragged set of rows:
+    ``y[r] = row_weight[r] * (x[r // top_k] @ w[e].T)`` for the rows r that
+    ``order`` holds at positions ``offsets[e]`` to ``offsets[e + 1]``
+    (``group_routes``); without ``order`` the rows are laid out by expert and
+    position i is row i.  ``x`` [rows, K] and ``w`` [E, N, K] are both bfloat16 (K a
+    multiple of 8), or both int8 (of 16) with ``x_scale`` [rows] and ``w_scale`` [E,
+    N] float32.  With an ``activation`` the first N/2 rows of each matrix are gate
+    and the others up rows, and the result is ``act(gate) * up``.  Returns bfloat16
+    [rows * top_k, N or N/2]; rows of no expert are not written (in a fresh
+    result they hold whatever the memory held)."""
+    if x.dtype not in (torch.bfloat16, torch.int8) or w.dtype != x.dtype:
+        raise ValueError("x and w must both be bfloat16 or both int8")
+    if x.dim() != 2 or w.dim() != 3 or x.shape[1] != w.shape[2]:
+        raise ValueError("x must be [rows, K] and w [experts, N, K]")
+    if top_k < 1 or (order is None and top_k != 1):
+        raise ValueError("top_k is 1 without an order, else positive")
+    (t, k), (e, n) = x.shape, w.shape[:2]
+    rows = t * top_k
+    if offsets.dtype != torch.int32 or tuple(offsets.shape) != (e + 1,):
+        raise ValueError("offsets must be int32 [experts + 1]")
+    if order is not None and (order.dtype != torch.int32 or order.numel() != rows):
+        raise ValueError("order must be int32 with one entry per row of the result")
+    int8 = x.dtype == torch.int8
+    if int8 != (x_scale is not None) or int8 != (w_scale is not None):
+        raise ValueError("int8 operands take x_scale and w_scale, bfloat16 ones none")
+    if int8 and (x_scale.dtype != torch.float32 or w_scale.dtype != torch.float32 or x_scale.shape != x.shape[:1]
+                 or w_scale.shape != w.shape[:2]):
+        raise ValueError("x_scale must be float32 [rows], w_scale float32 [experts, N]")
+    if row_weight is not None and (row_weight.dtype != torch.float32 or row_weight.numel() != rows):
+        raise ValueError("row_weight must be float32 with one entry per row of the result")
+    act = _act_code(activation)
+    tensors = (x, w, offsets, order, x_scale, w_scale, row_weight, out)
+    _require_gpu(*tensors)
+    dev = _one_device(*tensors)
+    shape = (rows, n if activation is None else n // 2)
+    if out is not None and (out.dtype != torch.bfloat16 or tuple(out.shape) != shape):
+        raise ValueError(f"out must be bfloat16 {shape}")
+    y = out if out is not None else torch.empty(shape, dtype=torch.bfloat16, device=dev)
+    g = _lib.FtmoeGrouped(_lib.FMT_INT8 if int8 else _lib.FMT_BF16, e, n, k, _ptr(x), _ptr(x_scale), _ptr(w),
+                          _ptr(w_scale), t, top_k, _ptr(offsets), _ptr(order), _ptr(row_weight), act, _ptr(y))
+    with torch.cuda.device(dev):
+        check(lib().ftmoe_grouped_matmul(ctypes.byref(g), _stream(dev)), "grouped_matmul")
+    return y
+
+
 # --------------------------------------------------------------------------- expert banks
 
-_FORMATS = {"bf16": _lib.FMT_BF16, "fp8_block": _lib.FMT_FP8_B128, "mxfp4": _lib.FMT_MXFP4}
+_FORMATS = {"bf16": _lib.FMT_BF16, "fp8_block": _lib.FMT_FP8_B128, "mxfp4": _lib.FMT_MXFP4, "int8": _lib.FMT_INT8}
 
 
 @dataclass
@@ -306,6 +442,8 @@ class ExpertBank:
     (or bf16, converted once) 128x128 block scales.
     fmt "mxfp4": uint8 packed [S,2I,H/2] / [S,H,I/2] with uint8 e8m0 scales
     [S,2I,H/32] / [S,H,I/32].
+    fmt "int8": int8 [S,2I,H] / [S,H,I] with float32 scales of the output
+    channels [S,2I] / [S,H] (``experts_int8``).
     ``swiglu_limit`` > 0 makes the activation the clamped SwiGLU
     ``silu(min(gate, L)) * clamp(up, -L, L)`` (DeepSeek-V4's experts,
     ``moe/fused_ds_fp4.py:105-124``); 0 leaves it unclamped.
@@ -330,6 +468,15 @@ class ExpertBank:
                     setattr(self, name, s.float().contiguous())
         if self.fmt == "bf16" and self.gate_up.dtype != torch.bfloat16:
             raise ValueError("bf16 bank weights must be torch.bfloat16")
+        if self.fmt == "int8":
+            if self.gate_up.dtype != torch.int8 or self.down.dtype != torch.int8:
+                raise ValueError("int8 bank weights must be torch.int8")
+            for w, s in ((self.gate_up, self.gate_up_scale), (self.down, self.down_scale)):
+                if s is None or s.dtype != torch.float32 or s.shape != w.shape[:2]:
+                    raise ValueError("int8 bank needs float32 scales [rows, output channels]")
+            rows, hidden, inter = self.down.shape
+            if tuple(self.gate_up.shape) != (rows, 2 * inter, hidden):
+                raise ValueError("int8 bank matrices are [rows, 2 inter, hidden] and [rows, hidden, inter]")
 
     @property
     def num_rows(self) -> int:
@@ -566,6 +713,55 @@ def experts_prefill(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.Tenso
                                     _ptr(y), _ptr(ws), ws.numel(), _stream(x.device)),
         "experts_prefill",
     )
+    return y
+
+
+def quantize_bank_int8(bank: ExpertBank) -> ExpertBank:
+    """The int8 bank of a bf16 one: every output channel of every expert gets
+    its own scale (``act_quant_int8`` of the weight rows)."""
+    if bank.fmt != "bf16":
+        raise ValueError(f"cannot quantise a {bank.fmt} bank to int8")
+    (gate_up, gs), (down, ds) = act_quant_int8(bank.gate_up), act_quant_int8(bank.down)
+    return ExpertBank("int8", gate_up, down, gs, ds, swiglu_limit=bank.swiglu_limit)
+
+
+def experts_int8(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.Tensor, bank: ExpertBank,
+                 shared: ExpertBank | None = None, activation: str = "silu",
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+    """Experts of an int8 bank (+ optional int8 shared expert) for a precomputed
+    routing, decode and prefill alike: 8-bit products with one scale per token
+    (per route between the two products) and per output channel (see
+    ftmoe_experts_int8).  Ids outside the bank's rows are skipped."""
+    if x.dtype != torch.bfloat16:
+        raise ValueError("hidden_states must be bfloat16")
+    if topk_w.dtype != torch.float32 or topk_ids.dtype != torch.int32:
+        raise ValueError("topk_weights must be float32 and topk_ids int32")
+    if topk_w.shape != topk_ids.shape or topk_ids.dim() != 2:
+        raise ValueError("topk shape mismatch")
+    if activation not in _lib.ACT:
+        raise ValueError(f"Unsupported activation: {activation}")
+    if bank.fmt != "int8" or (shared is not None and shared.fmt != "int8"):
+        raise ValueError("experts_int8 takes int8 banks")
+    _require_gpu(x, topk_w, topk_ids, out)
+    m, k = topk_ids.shape
+    if x.dim() != 2 or x.shape[0] != m:
+        raise ValueError("Number of tokens mismatch")
+    if x.shape[1] != bank.hidden:
+        raise ValueError("Hidden size mismatch")
+    if out is not None and (out.dtype != torch.bfloat16 or out.shape != x.shape):
+        raise ValueError("out must be bfloat16 shaped like hidden_states")
+    b = bank.cstruct()
+    sb = shared.cstruct() if shared is not None else None
+    bp = ctypes.byref(b)
+    sp = ctypes.byref(sb) if sb is not None else None
+    dev = _one_device(x, topk_w, topk_ids, out, bank.gate_up, bank.down, bank.gate_up_scale, bank.down_scale,
+                      *((shared.gate_up, shared.down, shared.gate_up_scale, shared.down_scale) if shared else ()))
+    # a workspace of the call's own: of the stream's pool, or of the graph's under capture
+    ws = torch.empty((lib().ftmoe_experts_int8_workspace(m, k, bp, sp),), dtype=torch.uint8, device=dev)
+    y = out if out is not None else torch.empty_like(x)
+    with torch.cuda.device(dev):
+        check(lib().ftmoe_experts_int8(_ptr(x), m, k, _ptr(topk_w), _ptr(topk_ids), bp, sp, _lib.ACT[activation],
+                                       _ptr(y), _ptr(ws), ws.numel(), _stream(dev)), "experts_int8")
     return y
 
 

@@ -50,10 +50,11 @@ enum ftmoe_format {
   FTMOE_FMT_NONE = -1,
   FTMOE_FMT_BF16 = 0,     /* bf16 weights */
   FTMOE_FMT_FP8_B128 = 1, /* e4m3 weights + float32 128x128 block scales */
-  FTMOE_FMT_MXFP4 = 2     /* e2m1 weights + e8m0 scale per 32 K (row-major "ds_fp4" layout) */
+  FTMOE_FMT_MXFP4 = 2,    /* e2m1 weights + e8m0 scale per 32 K (row-major "ds_fp4" layout) */
+  FTMOE_FMT_INT8 = 3      /* int8 weights + float32 scale per output channel (ftmoe_experts_int8, ftmoe_grouped_matmul) */
 };
 
-enum ftmoe_activation { FTMOE_ACT_SILU = 0, FTMOE_ACT_GELU = 1, FTMOE_ACT_GELU_TANH = 2 };
+enum ftmoe_activation { FTMOE_ACT_NONE = -1 /* matrix products only */, FTMOE_ACT_SILU = 0, FTMOE_ACT_GELU = 1, FTMOE_ACT_GELU_TANH = 2 };
 
 /* Indices of the int64 counters accumulated by ftmoe_slot_map (moe/offload_cache.py:205-229). */
 enum ftmoe_stat { FTMOE_STAT_ACTIVE = 0, FTMOE_STAT_MISS = 1, FTMOE_STAT_CALLS = 2, FTMOE_STAT_MISSED_ROUTES = 3 };
@@ -64,8 +65,9 @@ enum ftmoe_stat { FTMOE_STAT_ACTIVE = 0, FTMOE_STAT_MISS = 1, FTMOE_STAT_CALLS =
  *   FP8_B128: gate_up_scale float [S, 2I/128, H/128], down_scale float [S, H/128, I/128];
  *   MXFP4:    gate_up [S, 2I, H/2] bytes, gate_up_scale uint8 [S, 2I, H/32],
  *             down [S, H, I/2] bytes, down_scale uint8 [S, H, I/32];
- *   BF16:     scales NULL.
- * H and I must be multiples of 128. */
+ *   BF16:     scales NULL;
+ *   INT8:     gate_up [S, 2I, H] and down [S, H, I] int8, gate_up_scale float [S, 2I], down_scale float [S, H].
+ * H and I must be multiples of 128 (INT8: of 16). */
 typedef struct ftmoe_bank {
   int format;
   int num_rows;
@@ -329,6 +331,67 @@ size_t ftmoe_experts_prefill_workspace(int M, int top_k, const ftmoe_bank* bank,
 int ftmoe_experts_prefill(const void* x, int M, int top_k, const float* topk_w, const int32_t* topk_ids,
                           const ftmoe_bank* bank, const ftmoe_bank* shared, int activation, void* y,
                           void* workspace, size_t workspace_bytes, ftmoe_stream_t stream);
+
+/* ---- 8-bit integers and ragged groups (no counterpart in the reference) ----
+ * Rows of x and w start at 16-byte addresses and are whole 16-byte pieces: K is
+ * a multiple of 16 (int8) or 8 (bf16), and the pointers are 16-byte aligned. */
+
+/* Symmetric 8-bit quantisation with one scale per row.  x bf16 [rows, K]; with
+ * a the row's largest magnitude, q = round(127 x / a) (exactly, ties to even)
+ * int8 [rows, K] and scales = a / 127 float32 [rows]; x is about q * scale.  A
+ * row of zeros has scale 0; a row with an infinity or a NaN has scale NaN and
+ * codes 0, so that its products are NaN.  The rows may be a token's
+ * activations or a weight matrix's output channels. */
+int ftmoe_act_quant_int8(const void* x, int rows, int K, void* q, float* scales, ftmoe_stream_t stream);
+
+/* y[m, n] = q_scale[m] * w_scale[n] * sum_k q[m, k] w[n, k], the sum exact in
+ * 32-bit integers: q int8 [M, K], w int8 [N, K], scales float32, y [M, N] of
+ * out_dtype.  With an activation (not FTMOE_ACT_NONE) w holds N/2 gate rows,
+ * then N/2 up rows, and y [M, N/2] = act(gate) * up of those products in
+ * float32.  K <= 131056; x and one tile of w within 2 GiB. */
+int ftmoe_matmul_int8(const void* q, const float* q_scale, const void* w, const float* w_scale, int M, int N, int K,
+                      int activation, int out_dtype, void* y, ftmoe_stream_t stream);
+
+/* Routes in the order of their experts (stable): order int32 [numel] lists the
+ * flat route indices of expert 0, then expert 1, ..., then those with id ==
+ * num_experts; routes with other ids are left out, and the tail of order holds
+ * numel.  offsets int32 [num_experts + 2]: offsets[e] .. offsets[e + 1] are the
+ * positions of expert e; the last entry ends those of id num_experts.  This is
+ * ftmoe_align's order with block size 1.  num_experts <= 1023. */
+size_t ftmoe_group_routes_workspace(int numel, int num_experts);
+int ftmoe_group_routes(const int32_t* topk_ids, int numel, int num_experts, int32_t* order, int32_t* offsets,
+                       void* workspace, size_t workspace_bytes, ftmoe_stream_t stream);
+
+/* Matrix products grouped by expert, each with a ragged set of rows:
+ *   y[r] = row_weight[r] * (x[r / top_k] . w[e]^T)   for r = order[i] and offsets[e] <= i < offsets[e + 1],
+ * with the sums in float32 (bf16) or exact in 32-bit integers and scaled (int8). */
+typedef struct ftmoe_grouped {
+  int format;               /* FTMOE_FMT_BF16 or FTMOE_FMT_INT8: x and w */
+  int num_experts, N, K;
+  const void* x;            /* [x_rows, K] */
+  const float* x_scale;     /* int8: [x_rows] */
+  const void* w;            /* [num_experts, N, K] */
+  const float* w_scale;     /* int8: [num_experts, N] */
+  int x_rows;
+  int top_k;                /* rows of y per row of x; 1 without order */
+  const int32_t* offsets;   /* [num_experts + 1], ascending, within [0, x_rows * top_k]; device values outside are cut */
+  const int32_t* order;     /* nullable [x_rows * top_k]: y rows by group, each at most once; NULL: position i is row i */
+  const float* row_weight;  /* nullable [x_rows * top_k] */
+  int activation;           /* FTMOE_ACT_NONE, or as ftmoe_matmul_int8 */
+  void* y;                  /* bf16 [x_rows * top_k, N] (N/2 with an activation); rows of no group are left as they were */
+} ftmoe_grouped;
+int ftmoe_grouped_matmul(const ftmoe_grouped* args, ftmoe_stream_t stream);
+
+/* Expert layer of an INT8 bank for a precomputed routing, decode and prefill
+ * alike: tokens are quantised (ftmoe_act_quant_int8), multiplied with the gate
+ * and up rows, act(gate) * up is rounded to bf16 and quantised per route,
+ * multiplied with the down rows and the router weight, and the routes of a token
+ * (and the shared expert, nullable, an INT8 bank of one row) are summed in
+ * float32.  Ids outside [0, num_rows) are skipped.  num_rows <= 1023. */
+size_t ftmoe_experts_int8_workspace(int M, int top_k, const ftmoe_bank* bank, const ftmoe_bank* shared);
+int ftmoe_experts_int8(const void* x, int M, int top_k, const float* topk_w, const int32_t* topk_ids,
+                       const ftmoe_bank* bank, const ftmoe_bank* shared, int activation, void* y, void* workspace,
+                       size_t workspace_bytes, ftmoe_stream_t stream);
 
 /* Host-side expert executor of the hybrid decode (CPU pool computing the
  * routes whose experts are on the host; replaces the CPU MoE executor of the
