@@ -816,6 +816,9 @@ int check_product(const ftmoe::MatmulArgs& a, const char* what) {
   const size_t row = static_cast<size_t>(a.K) * (a.int8 ? 1 : 2), lim = size_t{1} << 31;
   if (row * a.x_rows >= lim || row * 256 >= lim)
     return fail(FTMOE_ERR_UNSUPPORTED, "%s: x of %d rows or 256 rows of w of K=%d reach 2 GiB", what, a.x_rows, a.K);
+  // (the gate and up rows of a tile are reached from one address)
+  if (a.act != FTMOE_ACT_NONE && row * a.N >= lim)
+    return fail(FTMOE_ERR_UNSUPPORTED, "%s: a gate and up matrix of %d rows of K=%d reaches 2 GiB", what, a.N, a.K);
   if (a.rows == 0) return FTMOE_OK;
   if (!a.x || !a.w || !a.y || (a.int8 && (!a.xs || !a.ws))) return fail(FTMOE_ERR_INVALID, "%s: NULL pointer", what);
   if (!aligned16(a.x) || !aligned16(a.w) || !aligned16(a.y))

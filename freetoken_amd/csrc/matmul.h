@@ -1,0 +1,71 @@
+// Pieces shared by the matrix products' kernels (matmul.hip, matmul_tile.hip).
+#pragma once
+
+#include "kernels.h"
+
+namespace ftmoe {
+
+typedef int acc_i32 __attribute__((ext_vector_type(4)));
+
+template <bool INT8>
+struct Acc {
+  using type = f32x4;
+};
+template <>
+struct Acc<true> {
+  using type = acc_i32;
+};
+
+template <bool INT8>
+__device__ __forceinline__ typename Acc<INT8>::type mma(u32x4 a, u32x4 b, typename Acc<INT8>::type c) {
+  if constexpr (INT8)
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                   0);
+}
+
+// 32 x 32 outputs from 32 bytes of K: a lane holds the 16 bytes of half l / 32 of
+// row l % 32, and results 8 (v / 4) + 4 (l / 32) + v % 4 (row of A), l % 32 (row of B).
+typedef int acc32_i32 __attribute__((ext_vector_type(16)));
+typedef float acc32_f32 __attribute__((ext_vector_type(16)));
+template <bool INT8>
+struct Acc32 {
+  using type = acc32_f32;
+};
+template <>
+struct Acc32<true> {
+  using type = acc32_i32;
+};
+
+template <bool INT8>
+__device__ __forceinline__ typename Acc32<INT8>::type mma32(u32x4 a, u32x4 b, typename Acc32<INT8>::type c) {
+  if constexpr (INT8)
+    return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                   0);
+}
+
+// Rows [begin, end) of group e in the grouped order, cut to [0, rows] whatever
+// the offsets hold.
+__device__ __forceinline__ void group_range(const MatmulArgs& a, int e, int& begin, int& end) {
+  if (!a.offsets) {
+    begin = 0;
+    end = a.rows;
+    return;
+  }
+  begin = min(max(a.offsets[e], 0), a.rows);
+  end = min(max(a.offsets[e + 1], begin), a.rows);
+}
+
+// The streaming form, for few rows per group (matmul_stream.hip); wide: 32 features x 32 rows per workgroup, else
+// 16 x 16.
+hipError_t launch_matmul_stream(const MatmulArgs& a, bool wide, hipStream_t stream);
+
+// The tiled form, for many rows per group (matmul_tile.hip): weight rows x rows of x of a workgroup; once: the weights
+// are read about once, past the caches.
+enum TileShape { kTile128x64, kTile256x128, kTile256x256 };
+hipError_t launch_matmul_tile(const MatmulArgs& a, TileShape shape, bool once, hipStream_t stream);
+
+}  // namespace ftmoe

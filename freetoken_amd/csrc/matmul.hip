@@ -1,131 +1,20 @@
-// Matrix products with one weight matrix per group of rows: dense int8 products
-// (one group) and the products grouped by expert, bf16 or int8 (MatmulArgs).
+// Matrix products with one weight matrix per group of rows (MatmulArgs): dense
+// int8 products (one group) and the products grouped by expert, bf16 or int8; and
+// the sum of an expert layer's routes.  Here: the choice between the streaming form
+// (matmul_stream.hip) and the tiled one (matmul_tile.hip).
 //
-// Weights are the MFMA A operand (rows = output features), rows of x the B
-// operand (columns).  Both types take 64 bytes of a row per MFMA: 32 bf16 values
-// (v_mfma_f32_16x16x32_bf16) or 64 int8 (v_mfma_i32_16x16x64_i8), a lane holding
-// the 16 bytes of lane group l / 16.  A and B use the same placement of K, so the
-// products pair up whatever the order inside the instruction.
+// In both, weights are the MFMA A operand (rows = output features), rows of x the B
+// operand (columns), and both types take 16 bytes of a row per lane: A and B use the same
+// placement of K, so the products pair up whatever the order inside the instruction.
+#include <cmath>
 #include <algorithm>
 
 #include "kernels.h"
+#include "matmul.h"
 
 namespace ftmoe {
 
-typedef int acc_i32 __attribute__((ext_vector_type(4)));
-
 namespace {
-
-template <bool INT8>
-struct Acc {
-  using type = f32x4;
-};
-template <>
-struct Acc<true> {
-  using type = acc_i32;
-};
-
-template <bool INT8>
-__device__ __forceinline__ typename Acc<INT8>::type mma(u32x4 a, u32x4 b, typename Acc<INT8>::type c) {
-  if constexpr (INT8)
-    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
-                                                   0);
-}
-
-// Rows [begin, end) of group e in the grouped order, cut to [0, rows] whatever
-// the offsets hold.
-__device__ __forceinline__ void group_range(const MatmulArgs& a, int e, int& begin, int& end) {
-  if (!a.offsets) {
-    begin = 0;
-    end = a.rows;
-    return;
-  }
-  begin = min(max(a.offsets[e], 0), a.rows);
-  end = min(max(a.offsets[e + 1], begin), a.rows);
-}
-
-// The group of block b of the grid's blocks of `block` rows (one wave: a scan of
-// the groups' block counts, 64 at a time); false past the last block.
-__device__ __forceinline__ bool find_block(const MatmulArgs& a, int block, int b, int& e, int& begin, int& end) {
-  const int lane = lane_id();
-  int done = 0;
-  for (int e0 = 0; e0 < a.E; e0 += kWave) {
-    int lo = 0, hi = 0;
-    if (e0 + lane < a.E) group_range(a, e0 + lane, lo, hi);
-    const int nb = (hi - lo + block - 1) / block;
-    int sum = nb;
-#pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) {
-      const int y = __shfl_up(sum, off, kWave);
-      if (lane >= off) sum += y;
-    }
-    const unsigned long long past = __ballot(done + sum > b);
-    if (past) {
-      const int l = __ffsll(static_cast<long long>(past)) - 1;
-      e = e0 + l;
-      const int first = done + __shfl(sum - nb, l, kWave);
-      begin = __shfl(lo, l, kWave) + (b - first) * block;
-      end = min(__shfl(hi, l, kWave), begin + block);
-      return true;
-    }
-    done += __shfl(sum, kWave - 1, kWave);
-  }
-  return false;
-}
-
-// One wave: 16 output features of 16 rows of one group.
-template <bool INT8>
-__global__ void __launch_bounds__(kWave) matmul_wave_kernel(MatmulArgs a) {
-  using acc_t = typename Acc<INT8>::type;
-  int e, begin, end;
-  if (!find_block(a, 16, blockIdx.y, e, begin, end)) return;
-  const int lane = lane_id(), r16 = lane & 15, g = lane >> 4;
-  const int n_out = a.act < 0 ? a.N : a.N / 2;
-  const int n0 = blockIdx.x * 16;
-  const size_t kb = static_cast<size_t>(a.K) * (INT8 ? 1 : 2);
-  // this lane's row of y
-  int r = -1;
-  if (begin + r16 < end) {
-    r = a.order ? a.order[begin + r16] : begin + r16;
-    if (r < 0 || r >= a.rows) r = -1;
-  }
-  const uint8_t* xr = a.x + static_cast<size_t>(r < 0 ? 0 : r / a.top_k) * kb;
-  const uint8_t* we = a.w + static_cast<size_t>(e) * a.N * kb;
-  const bool n_in = n0 + r16 < n_out;
-  const uint8_t* wg = we + static_cast<size_t>(n_in ? n0 + r16 : 0) * kb;
-  const uint8_t* wu = wg + static_cast<size_t>(n_out) * kb;
-  acc_t acc_g = {}, acc_u = {};
-  const u32x4 none = {0u, 0u, 0u, 0u};
-  for (size_t at = 0; at < kb; at += 64) {
-    const size_t c = at + 16 * g;
-    const bool in = c < kb;
-    const u32x4 xv = in && r >= 0 ? *reinterpret_cast<const u32x4*>(xr + c) : none;
-    acc_g = mma<INT8>(in && n_in ? *reinterpret_cast<const u32x4*>(wg + c) : none, xv, acc_g);
-    if (a.act >= 0) acc_u = mma<INT8>(in && n_in ? *reinterpret_cast<const u32x4*>(wu + c) : none, xv, acc_u);
-  }
-  if (r < 0) return;
-  const float xs = INT8 ? a.xs[r / a.top_k] : 1.0f;
-  const float rw = a.row_weight ? a.row_weight[r] : 1.0f;
-#pragma unroll
-  for (int v = 0; v < 4; ++v) {
-    const int n = n0 + 4 * g + v;
-    if (n >= n_out) break;
-    float o = static_cast<float>(acc_g[v]);
-    if constexpr (INT8) o *= a.ws[static_cast<size_t>(e) * a.N + n] * xs;
-    if (a.act >= 0) {
-      float u = static_cast<float>(acc_u[v]);
-      if constexpr (INT8) u *= a.ws[static_cast<size_t>(e) * a.N + n_out + n] * xs;
-      swiglu_clamp(a.limit, o, u);
-      o = act_apply(a.act, o) * u;
-    }
-    o *= rw;
-    const size_t at = static_cast<size_t>(r) * n_out + n;
-    if (a.out_f32) static_cast<float*>(a.y)[at] = o;
-    else static_cast<uint16_t*>(a.y)[at] = f32_to_bf16(o);
-  }
-}
 
 // y[t] = bf16(sum of the routes' rows in route order + shared[t]), routes with
 // ids outside [0, num_rows) skipped; H a multiple of 8.
@@ -160,13 +49,55 @@ __global__ void __launch_bounds__(256) combine_routes_kernel(const uint16_t* __r
 
 }  // namespace
 
+// Forms and tiles are chosen from the sizes known on the host: the rows per group
+// are R / E on average.  Measured (us, int8 unless said; stream 16 x 16 / stream 32 x 32 /
+// tiles of 128 x 64 / 256 x 128 / 256 x 256):
+//   one group, N 4096, K 7168: 1 row 7.1 / 9.9 / 22 / 38 / 72, 16 rows 8.4 / 10.6 / 22, 48 rows 19 / 12.6 / 22;
+//   N 7168, K 2048: 16 rows 6.5 / 5.7 / 10, 64 rows - / 9 / 10.5, 128 rows - / 15 / 10.7 / 16;
+//   8 rows over 128 experts, N 1536 (gate and up), K 2048: 9.1 / 9.9 / 14;
+//   bf16 32 rows over 128, N 1536 (gate and up), K 2048: 28 / 32 / 40; 100 rows over 256: 60 / 51 / 47;
+//   512 rows over 64, N 7168, K 2048: 209 / 158 / 147.
 hipError_t launch_matmul(const MatmulArgs& a, hipStream_t stream) {
-  const int n_out = a.act < 0 ? a.N : a.N / 2;
-  const int blocks = static_cast<int>(std::min<long long>(a.rows, a.rows / 16ll + a.E));
-  const dim3 grid((n_out + 15) / 16, blocks);
-  if (a.int8) hipLaunchKernelGGL(matmul_wave_kernel<true>, grid, dim3(kWave), 0, stream, a);
-  else hipLaunchKernelGGL(matmul_wave_kernel<false>, grid, dim3(kWave), 0, stream, a);
-  return hipGetLastError();
+  const long long n_out = a.act < 0 ? a.N : a.N / 2, rows = a.rows;
+  const long long row_bytes = static_cast<long long>(a.K) * (a.int8 ? 1 : 2);
+  if (rows <= 16ll * a.E) {
+    // the small workgroups win while they do not fill the chip, longer where their streams are long
+    const long long units = (n_out + 15) / 16 * std::min<long long>(rows, (rows + 15) / 16 + a.E - 1);
+    if (units <= 384 || (units <= 1536 && row_bytes >= 4096)) return launch_matmul_stream(a, false, stream);
+    if (units <= 1536) return launch_matmul_stream(a, true, stream);
+  } else if (a.E == 1 && rows <= 64) {
+    return launch_matmul_stream(a, true, stream);
+  }
+  // Tiles: the time of a shape goes by its rounds over the workgroups that fit the
+  // chip at once (the mean of the whole rounds and the fraction) times what a round
+  // of it takes, from the rates that large calls reach (dense 8192 x 4096 x 7168: 2320, 2140 and
+  // 1430 T/s).  Up to 32 rows per group the smallest tiles, whose weights pass
+  // the caches (1000 rows over 64 experts, N 7168, K 2048: 162, cached 176; 4000 rows 264 / 221);
+  // tiles of 128 rows read past the caches up to 64 (4000 rows 191 / 200, 8000 291 / 240).
+  if (rows <= 32ll * a.E && a.E > 1) return launch_matmul_tile(a, kTile128x64, true, stream);
+  struct Shape {
+    TileShape shape;
+    int feats, rows, slots;
+    double round;
+  };
+  constexpr Shape kShapes[] = {
+      {kTile128x64, 128, 64, 512, 11.5}, {kTile256x128, 256, 128, 256, 15.3}, {kTile256x256, 256, 256, 256, 28.3}};
+  const Shape* best = nullptr;
+  double least = 0;
+  for (const Shape& s : kShapes) {
+    const int feats = a.act < 0 ? s.feats : s.feats / 2;
+    // blocks of rows: a group's last one is half full on average
+    const double blocks = a.E == 1 ? static_cast<double>((rows + s.rows - 1) / s.rows)
+                                   : std::max<double>(std::min<long long>(rows, a.E),
+                                                      static_cast<double>(rows) / s.rows + 0.5 * a.E);
+    const double rounds = blocks * static_cast<double>((n_out + feats - 1) / feats) / s.slots;
+    const double t = 0.5 * (rounds + std::ceil(rounds)) * s.round;
+    if (!best || t < least) {
+      best = &s;
+      least = t;
+    }
+  }
+  return launch_matmul_tile(a, best->shape, best->shape == kTile256x128 && a.E > 1 && rows <= 64ll * a.E, stream);
 }
 
 hipError_t launch_combine_routes(const uint16_t* routes, const int32_t* ids, int num_rows, const float* shared, int M,

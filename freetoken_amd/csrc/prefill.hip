@@ -38,6 +38,7 @@
 #include <type_traits>
 
 #include "kernels.h"
+#include "lds_ring.h"
 #include "quant.h"
 
 namespace ftmoe {
@@ -381,7 +382,6 @@ __global__ void __launch_bounds__(kPThreads) prefill_gemm_kernel(PrefillGemmArgs
 // ----------------------------------------------------------------------------
 constexpr int kQRows = 256;   // weight rows per workgroup
 constexpr int kQThreads = 512;
-constexpr int kXcds = 8;
 constexpr int kQDynamicLds = 160 * 1024 - 4096;  // beside the tiles' route and weight lists
 // M blocks per chunk of the schedule (see map_tile_q): [FP8, MXFP4][gate_up, down].
 // Measured on C5 (interleaved A/B, ms): FP8 gate_up 4 -> 2.23-2.24, 8 -> 2.19-2.20,
@@ -435,41 +435,6 @@ struct QLds {
   using Blk = std::conditional_t<FMT == FMT_MXFP4 && BM == 256, uint16_t, int>;
   static_assert(kFixed + (kPrefillMaxRows + 1) * sizeof(Blk) <= kQDynamicLds, "the expert list fits beside the ring");
 };
-
-__device__ __forceinline__ int xcd_major(int b, int n) {
-  const int per = n / kXcds, rem = n % kXcds;
-  const int x = b % kXcds, i = b / kXcds;
-  return x * per + min(x, rem) + i;
-}
-
-struct MNTile {
-  int m, ntile;
-};
-
-// (M block, N tile) of position `local` in a group of nb M blocks x ntiles:
-// chunks of kQChunk M blocks, each chunk sweeping all N tiles.
-// (Returned by value, and from one call per mapping: results written through
-// references from two calls lived in scratch memory, whose loads wait for the
-// copies in flight.)
-template <int kQChunk>
-__device__ __forceinline__ MNTile chunked(int local, int nb, int ntiles) {
-  const int full = nb / kQChunk, rem = nb - full * kQChunk;
-  const int span = kQChunk * ntiles;
-  const bool whole = local < full * span;
-  const int c = whole ? local / span : full;
-  const int w = local - c * span, in = whole ? kQChunk : rem;
-  const int ntile = w / in;
-  return {c * kQChunk + (w - ntile * in), ntile};
-}
-
-// Lane index as an asm result: the compiler can neither hoist nor merge it,
-// so per-tile set-up code recomputes its lane-derived values instead of keeping
-// them live (or spilled) across the K loop.
-__device__ __forceinline__ int fresh_lane() {
-  int l;
-  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
-  return l;
-}
 
 struct QTile {
   bool shared;  // the shared expert's blocks (tokens in order) instead of a routed expert's
@@ -533,29 +498,6 @@ __device__ __forceinline__ bool map_tile_q(const PrefillGemmArgs& a, const Blk* 
   return true;
 }
 
-// s_barrier without the memory fence of __syncthreads (which would wait for
-// every copy in flight); the clobber keeps the compiler from moving LDS
-// accesses across it.
-__device__ __forceinline__ void bare_barrier() { asm volatile("s_barrier" ::: "memory"); }
-
-template <int N>
-__device__ __forceinline__ void wait_vm() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-
-__device__ __forceinline__ void wait_lgkm0() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
-
-// LDS-DMA copies through a buffer descriptor: each lane's 16 (4) bytes at lane
-// offset voff plus the wave-uniform soff land at dst + lane * 16 (4), dst
-// wave-uniform; a lane offset at or past the descriptor's range reads zeros
-// without memory traffic.
-__device__ __forceinline__ void lds_buf16(__amdgpu_buffer_rsrc_t r, uint8_t* dst, uint32_t voff, uint32_t soff) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)dst, 16, voff, soff, 0, 0);
-}
-__device__ __forceinline__ void lds_buf4(__amdgpu_buffer_rsrc_t r, uint8_t* dst, uint32_t voff, uint32_t soff) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)dst, 4, voff, soff, 0, 0);
-}
-
 // Chunk swizzles of the LDS lines, chosen by measurement (rocprofv3
 // SQ_LDS_BANK_CONFLICT over ds_read_b128 patterns on gfx950): for 128-byte
 // lines read as chunk pairs (2g, 2g+1) -- the FP8 and bf16 operands -- position
@@ -563,24 +505,9 @@ __device__ __forceinline__ void lds_buf4(__amdgpu_buffer_rsrc_t r, uint8_t* dst,
 // read as chunks (g, 4+g) -- the MXFP4 activations -- c ^ (line & 7) is
 // conflict-free; for 64-byte lines read as chunk g -- the MXFP4 weights --
 // c ^ ((line >> 1) & 3) is.
-__device__ __forceinline__ int swz_pair(int line) { return ((line & 3) << 1) | ((line >> 2) & 1); }
 template <int FMT>
 __device__ __forceinline__ int swz_b(int line) { return FMT == FMT_MXFP4 ? (line & 7) : swz_pair(line); }
 __device__ __forceinline__ int swz64(int line) { return (line >> 1) & 3; }
-
-// Position of a running count in a ring of N.  (Unsigned: the signed remainders
-// were a dozen more scalar operations at the head of every step, before its
-// first LDS read; FP8 calls gained 0.3-0.8%.)
-template <int N>
-__device__ __forceinline__ int ring(int i) {
-  return static_cast<int>(static_cast<unsigned>(i) % N);
-}
-
-// Empty asm that keeps the value's update at this point of the instruction
-// stream (no code is emitted).
-__device__ __forceinline__ void pin(f32x4& v) { asm volatile("" : "+v"(v)); }
-
-__device__ __forceinline__ uint64_t uniform_u64(uint64_t v) { return readlane_u64(v, 0); }
 
 template <int FMT, int GATE_UP, int BM, bool NT>
 __global__ void __launch_bounds__(kQThreads) prefill_qgemm_kernel(PrefillGemmArgs a) {

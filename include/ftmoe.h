@@ -348,7 +348,7 @@ int ftmoe_act_quant_int8(const void* x, int rows, int K, void* q, float* scales,
  * 32-bit integers: q int8 [M, K], w int8 [N, K], scales float32, y [M, N] of
  * out_dtype.  With an activation (not FTMOE_ACT_NONE) w holds N/2 gate rows,
  * then N/2 up rows, and y [M, N/2] = act(gate) * up of those products in
- * float32.  K <= 131056; x and one tile of w within 2 GiB. */
+ * float32.  K <= 131056; x, and with an activation w, below 2 GiB. */
 int ftmoe_matmul_int8(const void* q, const float* q_scale, const void* w, const float* w_scale, int M, int N, int K,
                       int activation, int out_dtype, void* y, ftmoe_stream_t stream);
 
