@@ -846,42 +846,10 @@ int check_int8_bank(const ftmoe_bank* b, const char* name, bool shared) {
   return FTMOE_OK;
 }
 
-// Routes up to which one workgroup groups them; more are counted by several.
-constexpr int kGroupOneWorkgroup = 4096;
-
-struct GroupLayout {
-  int32_t* total;
-  int32_t* gcount;
-  size_t bytes;
-};
-
-GroupLayout group_layout(void* ws, int numel, int num_experts) {
-  GroupLayout L{};
-  Carver c{static_cast<uint8_t*>(ws)};
-  L.total = c.take<int32_t>(1);
-  L.gcount = c.take<int32_t>(ftmoe::align_gcount_ints(numel, num_experts));
-  L.bytes = c.off;
-  return L;
-}
-
-hipError_t launch_group_routes(const int32_t* ids, int numel, int num_experts, int32_t* order, int32_t* offsets,
-                               const GroupLayout& L, ftmoe_stream_t stream) {
-  ftmoe::AlignArgs a{};
-  a.ids = ids;
-  a.numel = numel;
-  a.num_experts = num_experts;
-  a.block_size = 1;
-  a.sorted_ids = order;
-  a.max_padded = numel;
-  a.ntpp = L.total;
-  a.cum_out = offsets;
-  return numel <= kGroupOneWorkgroup ? ftmoe::launch_align(a, stream) : ftmoe::launch_align_large(a, L.gcount, stream);
-}
-
 struct Int8Layout {
   int32_t* order;
   int32_t* offsets;
-  GroupLayout group;
+  int32_t* hist;
   int8_t* xq;
   float* xs;
   uint16_t* act;    // [routes, inter], then the shared expert's [M, inter]
@@ -902,8 +870,7 @@ Int8Layout int8_layout(void* ws, int M, int k, const ftmoe_bank* bank, const ftm
   const size_t H = bank->hidden, I = bank->inter;
   L.order = c.take<int32_t>(numel);
   L.offsets = c.take<int32_t>(bank->num_rows + 2);
-  L.group = group_layout(ws ? static_cast<uint8_t*>(ws) + c.off : nullptr, numel, bank->num_rows);
-  c.off += L.group.bytes;
+  L.hist = c.take<int32_t>(ftmoe::group_hist_ints(numel, bank->num_rows));
   L.xq = c.take<int8_t>(M * H);
   L.xs = c.take<float>(M);
   L.act = c.take<uint16_t>(numel * I);
@@ -963,7 +930,7 @@ int ftmoe_matmul_int8(const void* q, const float* q_scale, const void* w, const 
 
 size_t ftmoe_group_routes_workspace(int numel, int num_experts) {
   if (numel < 0 || num_experts <= 0) return 0;
-  return group_layout(nullptr, numel, num_experts).bytes;
+  return round_up(std::max<size_t>(1, ftmoe::group_hist_ints(numel, num_experts) * sizeof(int32_t)));
 }
 
 int ftmoe_group_routes(const int32_t* topk_ids, int numel, int num_experts, int32_t* order, int32_t* offsets,
@@ -972,12 +939,16 @@ int ftmoe_group_routes(const int32_t* topk_ids, int numel, int num_experts, int3
   if (num_experts <= 0 || num_experts > ftmoe::kCountMaxRows)
     return fail(FTMOE_ERR_UNSUPPORTED, "group_routes: num_experts=%d (1 to %d)", num_experts, ftmoe::kCountMaxRows);
   if (((!topk_ids || !order) && numel) || !offsets) return fail(FTMOE_ERR_INVALID, "group_routes: NULL pointer");
-  const size_t need = group_layout(nullptr, numel, num_experts).bytes;
+  const size_t need = ftmoe_group_routes_workspace(numel, num_experts);
   if (!workspace || workspace_bytes < need)
     return fail(FTMOE_ERR_WORKSPACE, "group_routes: workspace %zu < %zu bytes", workspace_bytes, need);
-  return check_hip(launch_group_routes(topk_ids, numel, num_experts, order, offsets,
-                                       group_layout(workspace, numel, num_experts), stream),
-                   "group_routes launch");
+  ftmoe::GroupArgs a{};
+  a.ids = topk_ids;
+  a.numel = numel;
+  a.num_experts = num_experts;
+  a.order = order;
+  a.offsets = offsets;
+  return check_hip(ftmoe::launch_group_routes(a, static_cast<int32_t*>(workspace), stream), "group_routes launch");
 }
 
 int ftmoe_grouped_matmul(const ftmoe_grouped* g, ftmoe_stream_t stream) {
@@ -1106,11 +1077,18 @@ int ftmoe_experts_int8(const void* x, int M, int top_k, const float* topk_w, con
     if (rc == FTMOE_OK) rc = check_hip(err, what);
     return rc == FTMOE_OK;
   };
-  if (!run(launch_group_routes(topk_ids, numel, bank->num_rows, L.order, L.offsets, L.group, stream),
-           "experts_int8 grouping"))
-    return rc;
-  if (!run(ftmoe::launch_act_quant_int8(static_cast<const uint16_t*>(x), M, H, L.xq, L.xs, stream), "experts_int8 x quant"))
-    return rc;
+  ftmoe::GroupArgs g{};
+  g.ids = topk_ids;
+  g.numel = numel;
+  g.num_experts = bank->num_rows;
+  g.order = L.order;
+  g.offsets = L.offsets;
+  g.x = static_cast<const uint16_t*>(x);
+  g.x_rows = M;
+  g.K = H;
+  g.q = L.xq;
+  g.scales = L.xs;
+  if (!run(ftmoe::launch_group_routes(g, L.hist, stream), "experts_int8 grouping and x quant")) return rc;
   if (!run(ftmoe::launch_matmul(up, stream), "experts_int8 gate_up")) return rc;
   // (rows of skipped routes hold what the workspace held: quantised, never multiplied)
   if (!run(ftmoe::launch_act_quant_int8(L.act, numel, bank->inter, L.actq, L.as, stream), "experts_int8 act quant"))

@@ -296,6 +296,20 @@ struct MatmulArgs {
 };
 hipError_t launch_matmul(const MatmulArgs& a, hipStream_t stream);
 hipError_t launch_act_quant_int8(const uint16_t* x, int rows, int K, int8_t* q, float* scales, hipStream_t stream);
+// Routes by expert (group.hip), and beside it the quantisation of the tokens where x is given.
+struct GroupArgs {
+  const int32_t* ids;     // [numel]
+  int numel, num_experts; // num_experts <= kCountMaxRows
+  int32_t* order;         // [numel]
+  int32_t* offsets;       // [num_experts + 2]
+  const uint16_t* x;      // nullable [x_rows, K] bf16 -> q [x_rows, K], scales [x_rows]
+  int x_rows, K;
+  int8_t* q;
+  float* scales;
+};
+size_t group_hist_ints(int numel, int num_experts);  // workspace of launch_group_routes
+hipError_t launch_group_routes(const GroupArgs& a, int32_t* hist, hipStream_t stream);
+
 // The routes' rows of every token (ids outside [0, num_rows) skipped) and its float32 shared row (nullable), summed
 // in float32 and rounded once.
 hipError_t launch_combine_routes(const uint16_t* routes, const int32_t* ids, int num_rows, const float* shared, int M,

@@ -6,8 +6,8 @@
 // In both, weights are the MFMA A operand (rows = output features), rows of x the B
 // operand (columns), and both types take 16 bytes of a row per lane: A and B use the same
 // placement of K, so the products pair up whatever the order inside the instruction.
-#include <cmath>
 #include <algorithm>
+#include <cmath>
 
 #include "kernels.h"
 #include "matmul.h"
@@ -16,25 +16,41 @@ namespace ftmoe {
 
 namespace {
 
+constexpr int kCombineThreads = 64;  // (a decode step has few: spread over the CUs)
+
 // y[t] = bf16(sum of the routes' rows in route order + shared[t]), routes with
-// ids outside [0, num_rows) skipped; H a multiple of 8.
-__global__ void __launch_bounds__(256) combine_routes_kernel(const uint16_t* __restrict__ routes,
-                                                             const int32_t* __restrict__ ids, int num_rows,
-                                                             const float* __restrict__ shared, int M, int k, int H,
-                                                             uint16_t* __restrict__ y) {
-  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+// ids outside [0, num_rows) skipped; H a multiple of 8.  The rows of eight routes
+// are read before the first is added.
+__global__ void __launch_bounds__(kCombineThreads) combine_routes_kernel(const uint16_t* __restrict__ routes,
+                                                                         const int32_t* __restrict__ ids, int num_rows,
+                                                                         const float* __restrict__ shared, int M, int k,
+                                                                         int H, uint16_t* __restrict__ y) {
+  const long long i = static_cast<long long>(blockIdx.x) * kCombineThreads + threadIdx.x;
   const int per = H / 8;
   if (i >= static_cast<long long>(M) * per) return;
   const int t = static_cast<int>(i / per), h = static_cast<int>(i % per) * 8;
+  const int32_t* const tid = ids + static_cast<size_t>(t) * k;
+  const uint16_t* const first = routes + static_cast<size_t>(t) * k * H + h;
   float acc[8] = {};
-  for (int j = 0; j < k; ++j) {
-    const int e = ids[static_cast<size_t>(t) * k + j];
-    if (e < 0 || e >= num_rows) continue;
-    const u32x4 v = *reinterpret_cast<const u32x4*>(routes + (static_cast<size_t>(t) * k + j) * H + h);
+  for (int j0 = 0; j0 < k; j0 += 8) {
+    u32x4 v[8];
+    bool in[8];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      acc[2 * w] += __uint_as_float(v[w] << 16);
-      acc[2 * w + 1] += __uint_as_float(v[w] & 0xffff0000u);
+    for (int j = 0; j < 8; ++j) {
+      const int e = j0 + j < k ? tid[j0 + j] : -1;
+      in[j] = e >= 0 && e < num_rows;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (in[j]) v[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(first + static_cast<size_t>(j0 + j) * H));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (!in[j]) continue;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        acc[2 * w] += __uint_as_float(v[j][w] << 16);
+        acc[2 * w + 1] += __uint_as_float(v[j][w] & 0xffff0000u);
+      }
     }
   }
   if (shared) {
@@ -103,7 +119,7 @@ hipError_t launch_matmul(const MatmulArgs& a, hipStream_t stream) {
 hipError_t launch_combine_routes(const uint16_t* routes, const int32_t* ids, int num_rows, const float* shared, int M,
                                  int k, int H, uint16_t* y, hipStream_t stream) {
   const long long n = static_cast<long long>(M) * (H / 8);
-  hipLaunchKernelGGL(combine_routes_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, stream, routes,
+  hipLaunchKernelGGL(combine_routes_kernel, dim3(static_cast<unsigned>((n + kCombineThreads - 1) / kCombineThreads)), dim3(kCombineThreads), 0, stream, routes,
                      ids, num_rows, shared, M, k, H, y);
   return hipGetLastError();
 }

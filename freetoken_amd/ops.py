@@ -295,12 +295,22 @@ def act_quant_fp8(x: torch.Tensor, mode: int = 0):
 # --------------------------------------------------------------------------- 8-bit integers, ragged groups
 
 
-def _one_device(*tensors: torch.Tensor | None) -> torch.device:
+def _one_device(first: torch.Tensor, *others: torch.Tensor | None) -> torch.device:
     """The device that holds all the tensors."""
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) != 1:
-        raise ValueError(f"tensors on different devices: {sorted(map(str, devices))}")
-    return devices.pop()
+    dev = first.device
+    for t in others:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on different devices: {dev} and {t.device}")
+    return dev
+
+
+def _launch(what: str, fn, dev: torch.device, *args) -> None:
+    """Calls the entry point with ``dev`` current and its current stream last."""
+    if torch._C._cuda_getDevice() == dev.index:  # (the guard object costs 1.4 us a call)
+        check(fn(*args, _stream(dev)), what)
+    else:
+        with torch.cuda.device(dev):
+            check(fn(*args, _stream(dev)), what)
 
 
 def _act_code(activation: str | None) -> int:
@@ -323,9 +333,7 @@ def act_quant_int8(x: torch.Tensor):
     _require_gpu(x)
     q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
     s = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
-        check(lib().ftmoe_act_quant_int8(_ptr(x), s.numel(), x.shape[-1], _ptr(q), _ptr(s), _stream(x.device)),
-              "act_quant_int8")
+    _launch("act_quant_int8", lib().ftmoe_act_quant_int8, x.device, _ptr(x), s.numel(), x.shape[-1], _ptr(q), _ptr(s))
     return q, s
 
 
@@ -353,10 +361,8 @@ def matmul_int8(q: torch.Tensor, q_scale: torch.Tensor, w: torch.Tensor, w_scale
         raise ValueError("the result is bfloat16 or float32")
     if tuple(y.shape) != shape:
         raise ValueError(f"out must be {shape}")
-    with torch.cuda.device(dev):
-        check(lib().ftmoe_matmul_int8(_ptr(q), _ptr(q_scale), _ptr(w), _ptr(w_scale), m, n, k, act,
-                                      _lib.DTYPE_F32 if y.dtype == torch.float32 else _lib.DTYPE_BF16, _ptr(y),
-                                      _stream(dev)), "matmul_int8")
+    _launch("matmul_int8", lib().ftmoe_matmul_int8, dev, _ptr(q), _ptr(q_scale), _ptr(w), _ptr(w_scale), m, n, k, act,
+            _lib.DTYPE_F32 if y.dtype == torch.float32 else _lib.DTYPE_BF16, _ptr(y))
     return y
 
 
@@ -373,9 +379,8 @@ def group_routes(topk_ids: torch.Tensor, num_experts: int):
     order = torch.empty((numel,), dtype=torch.int32, device=dev)
     offsets = torch.empty((max(num_experts, 0) + 2,), dtype=torch.int32, device=dev)
     ws = torch.empty((lib().ftmoe_group_routes_workspace(numel, num_experts),), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        check(lib().ftmoe_group_routes(_ptr(topk_ids), numel, num_experts, _ptr(order), _ptr(offsets), _ptr(ws),
-                                       ws.numel(), _stream(dev)), "group_routes")
+    _launch("group_routes", lib().ftmoe_group_routes, dev, _ptr(topk_ids), numel, num_experts, _ptr(order),
+            _ptr(offsets), _ptr(ws), ws.numel())
     return order, offsets[: num_experts + 1]
 
 
@@ -423,8 +428,7 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, orde
     y = out if out is not None else torch.empty(shape, dtype=torch.bfloat16, device=dev)
     g = _lib.FtmoeGrouped(_lib.FMT_INT8 if int8 else _lib.FMT_BF16, e, n, k, _ptr(x), _ptr(x_scale), _ptr(w),
                           _ptr(w_scale), t, top_k, _ptr(offsets), _ptr(order), _ptr(row_weight), act, _ptr(y))
-    with torch.cuda.device(dev):
-        check(lib().ftmoe_grouped_matmul(ctypes.byref(g), _stream(dev)), "grouped_matmul")
+    _launch("grouped_matmul", lib().ftmoe_grouped_matmul, dev, ctypes.byref(g))
     return y
 
 
@@ -759,9 +763,8 @@ def experts_int8(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.Tensor, 
     # a workspace of the call's own: of the stream's pool, or of the graph's under capture
     ws = torch.empty((lib().ftmoe_experts_int8_workspace(m, k, bp, sp),), dtype=torch.uint8, device=dev)
     y = out if out is not None else torch.empty_like(x)
-    with torch.cuda.device(dev):
-        check(lib().ftmoe_experts_int8(_ptr(x), m, k, _ptr(topk_w), _ptr(topk_ids), bp, sp, _lib.ACT[activation],
-                                       _ptr(y), _ptr(ws), ws.numel(), _stream(dev)), "experts_int8")
+    _launch("experts_int8", lib().ftmoe_experts_int8, dev, _ptr(x), m, k, _ptr(topk_w), _ptr(topk_ids), bp, sp,
+            _lib.ACT[activation], _ptr(y), _ptr(ws), ws.numel())
     return y
 
 
