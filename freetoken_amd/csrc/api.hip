@@ -852,14 +852,10 @@ struct Int8Layout {
   int32_t* hist;
   int8_t* xq;
   float* xs;
-  uint16_t* act;    // [routes, inter], then the shared expert's [M, inter]
+  uint16_t* act;     // [routes, inter], then the shared expert's [M, its inter]
   int8_t* actq;
-  float* as;
-  uint16_t* routes;  // [routes, hidden]
-  uint16_t* sh_act;
-  int8_t* sh_actq;
-  float* sh_as;
-  float* sh_out;     // [M, hidden]
+  float* as;         // [routes + M]
+  uint16_t* routes;  // [routes + M, hidden]
   size_t bytes;
 };
 
@@ -867,23 +863,17 @@ Int8Layout int8_layout(void* ws, int M, int k, const ftmoe_bank* bank, const ftm
   Int8Layout L{};
   Carver c{static_cast<uint8_t*>(ws)};
   const int numel = M * k;
-  const size_t H = bank->hidden, I = bank->inter;
+  const size_t H = bank->hidden, rows = numel + static_cast<size_t>(shared ? M : 0);
+  const size_t act = static_cast<size_t>(numel) * bank->inter + (shared ? static_cast<size_t>(M) * shared->inter : 0);
   L.order = c.take<int32_t>(numel);
   L.offsets = c.take<int32_t>(bank->num_rows + 2);
   L.hist = c.take<int32_t>(ftmoe::group_hist_ints(numel, bank->num_rows));
   L.xq = c.take<int8_t>(M * H);
   L.xs = c.take<float>(M);
-  L.act = c.take<uint16_t>(numel * I);
-  L.actq = c.take<int8_t>(numel * I);
-  L.as = c.take<float>(numel);
-  L.routes = c.take<uint16_t>(numel * H);
-  if (shared) {
-    const size_t Is = shared->inter;
-    L.sh_act = c.take<uint16_t>(M * Is);
-    L.sh_actq = c.take<int8_t>(M * Is);
-    L.sh_as = c.take<float>(M);
-    L.sh_out = c.take<float>(M * H);
-  }
+  L.act = c.take<uint16_t>(act);
+  L.actq = c.take<int8_t>(act);
+  L.as = c.take<float>(rows);
+  L.routes = c.take<uint16_t>(rows * H);
   L.bytes = c.off;
   return L;
 }
@@ -1043,12 +1033,21 @@ int ftmoe_experts_int8(const void* x, int M, int top_k, const float* topk_w, con
   down.act = FTMOE_ACT_NONE;
   down.row_weight = topk_w;
   down.y = L.routes;
-  for (const ftmoe::MatmulArgs* a : {&up, &down}) {
-    rc = check_product(*a, "experts_int8");
-    if (rc) return rc;
-  }
+  // The shared expert: one more group of both products where its matrices have the
+  // routed shape, else products of its own.
+  const bool joined = shared && shared->inter == bank->inter;
   ftmoe::MatmulArgs sh_up = up, sh_down = down;
-  if (shared) {
+  if (joined) {
+    up.extra = down.extra = M;
+    up.extra_w = static_cast<const uint8_t*>(shared->gate_up);
+    up.extra_ws = static_cast<const float*>(shared->gate_up_scale);
+    up.extra_limit = shared->swiglu_limit;
+    down.extra_x = numel;
+    down.extra_w = static_cast<const uint8_t*>(shared->down);
+    down.extra_ws = static_cast<const float*>(shared->down_scale);
+    down.x_rows = numel + M;
+  } else if (shared) {
+    const size_t at = static_cast<size_t>(numel) * bank->inter;
     sh_up.w = static_cast<const uint8_t*>(shared->gate_up);
     sh_up.ws = static_cast<const float*>(shared->gate_up_scale);
     sh_up.E = sh_down.E = 1;
@@ -1058,19 +1057,18 @@ int ftmoe_experts_int8(const void* x, int M, int top_k, const float* topk_w, con
     sh_up.rows = sh_down.rows = sh_down.x_rows = M;
     sh_up.top_k = 1;
     sh_up.limit = shared->swiglu_limit;
-    sh_up.y = L.sh_act;
-    sh_down.x = reinterpret_cast<const uint8_t*>(L.sh_actq);
-    sh_down.xs = L.sh_as;
+    sh_up.y = L.act + at;
+    sh_down.x = reinterpret_cast<const uint8_t*>(L.actq + at);
+    sh_down.xs = L.as + numel;
     sh_down.w = static_cast<const uint8_t*>(shared->down);
     sh_down.ws = static_cast<const float*>(shared->down_scale);
     sh_down.K = shared->inter;
     sh_down.row_weight = nullptr;
-    sh_down.out_f32 = 1;
-    sh_down.y = L.sh_out;
-    for (const ftmoe::MatmulArgs* a : {&sh_up, &sh_down}) {
-      rc = check_product(*a, "experts_int8");
-      if (rc) return rc;
-    }
+    sh_down.y = L.routes + static_cast<size_t>(numel) * H;
+  }
+  for (const ftmoe::MatmulArgs* a : {&up, &down, &sh_up, &sh_down}) {
+    rc = check_product(*a, "experts_int8");
+    if (rc) return rc;
   }
 
   const auto run = [&](hipError_t err, const char* what) {
@@ -1091,17 +1089,19 @@ int ftmoe_experts_int8(const void* x, int M, int top_k, const float* topk_w, con
   if (!run(ftmoe::launch_group_routes(g, L.hist, stream), "experts_int8 grouping and x quant")) return rc;
   if (!run(ftmoe::launch_matmul(up, stream), "experts_int8 gate_up")) return rc;
   // (rows of skipped routes hold what the workspace held: quantised, never multiplied)
-  if (!run(ftmoe::launch_act_quant_int8(L.act, numel, bank->inter, L.actq, L.as, stream), "experts_int8 act quant"))
+  if (!run(ftmoe::launch_act_quant_int8(L.act, numel + (joined ? M : 0), bank->inter, L.actq, L.as, stream),
+           "experts_int8 act quant"))
     return rc;
   if (!run(ftmoe::launch_matmul(down, stream), "experts_int8 down")) return rc;
-  if (shared) {
+  if (shared && !joined) {
+    const size_t at = static_cast<size_t>(numel) * bank->inter;
     if (!run(ftmoe::launch_matmul(sh_up, stream), "experts_int8 shared gate_up")) return rc;
-    if (!run(ftmoe::launch_act_quant_int8(L.sh_act, M, shared->inter, L.sh_actq, L.sh_as, stream),
+    if (!run(ftmoe::launch_act_quant_int8(L.act + at, M, shared->inter, L.actq + at, L.as + numel, stream),
              "experts_int8 shared act quant"))
       return rc;
     if (!run(ftmoe::launch_matmul(sh_down, stream), "experts_int8 shared down")) return rc;
   }
-  run(ftmoe::launch_combine_routes(L.routes, topk_ids, bank->num_rows, L.sh_out, M, top_k, H,
+  run(ftmoe::launch_combine_routes(L.routes, topk_ids, bank->num_rows, shared != nullptr, M, top_k, H,
                                    static_cast<uint16_t*>(y), stream),
       "experts_int8 combine");
   return rc;

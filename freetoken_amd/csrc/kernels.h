@@ -291,8 +291,14 @@ struct MatmulArgs {
   const float* row_weight;  // nullable [rows]
   int act;                  // -1: none, else Act
   float limit;              // clamped SwiGLU (> 0), else 0
+  // One more group, the shared expert's: rows [rows, rows + extra) of y, with a matrix of its own [N, K] and
+  // rows extra_x .. of x, without order and weights.
+  int extra, extra_x;
+  const uint8_t* extra_w;
+  const float* extra_ws;
+  float extra_limit;
   int out_f32;              // y float32 instead of bf16
-  void* y;                  // [rows, N] ([rows, N/2] with act)
+  void* y;                  // [rows + extra, N] (N/2 with act)
 };
 hipError_t launch_matmul(const MatmulArgs& a, hipStream_t stream);
 hipError_t launch_act_quant_int8(const uint16_t* x, int rows, int K, int8_t* q, float* scales, hipStream_t stream);
@@ -310,9 +316,9 @@ struct GroupArgs {
 size_t group_hist_ints(int numel, int num_experts);  // workspace of launch_group_routes
 hipError_t launch_group_routes(const GroupArgs& a, int32_t* hist, hipStream_t stream);
 
-// The routes' rows of every token (ids outside [0, num_rows) skipped) and its float32 shared row (nullable), summed
-// in float32 and rounded once.
-hipError_t launch_combine_routes(const uint16_t* routes, const int32_t* ids, int num_rows, const float* shared, int M,
+// The routes' rows of every token (ids outside [0, num_rows) skipped) and with shared its row behind all of those,
+// M k + t, summed in float32 and rounded once.
+hipError_t launch_combine_routes(const uint16_t* routes, const int32_t* ids, int num_rows, bool shared, int M,
                                  int k, int H, uint16_t* y, hipStream_t stream);
 
 hipError_t launch_combine(const uint16_t* ic3, const int32_t* ids, int num_rows, const uint16_t* sh_out, int M,

@@ -48,16 +48,21 @@ __device__ __forceinline__ typename Acc32<INT8>::type mma32(u32x4 a, u32x4 b, ty
 }
 
 // Rows [begin, end) of group e in the grouped order, cut to [0, rows] whatever
-// the offsets hold.
+// the offsets hold; group E is the extra one.
 __device__ __forceinline__ void group_range(const MatmulArgs& a, int e, int& begin, int& end) {
-  if (!a.offsets) {
+  if (e == a.E) {
+    begin = a.rows;
+    end = a.rows + a.extra;
+  } else if (!a.offsets) {
     begin = 0;
     end = a.rows;
-    return;
+  } else {
+    begin = min(max(a.offsets[e], 0), a.rows);
+    end = min(max(a.offsets[e + 1], begin), a.rows);
   }
-  begin = min(max(a.offsets[e], 0), a.rows);
-  end = min(max(a.offsets[e + 1], begin), a.rows);
 }
+
+__host__ __device__ inline int group_count(const MatmulArgs& a) { return a.E + (a.extra > 0 ? 1 : 0); }
 
 // The streaming form, for few rows per group (matmul_stream.hip); wide: 32 features x 32 rows per workgroup, else
 // 16 x 16.

@@ -18,13 +18,13 @@ namespace {
 
 constexpr int kCombineThreads = 64;  // (a decode step has few: spread over the CUs)
 
-// y[t] = bf16(sum of the routes' rows in route order + shared[t]), routes with
-// ids outside [0, num_rows) skipped; H a multiple of 8.  The rows of eight routes
-// are read before the first is added.
+// y[t] = bf16(sum of the routes' rows in route order, then the shared row M k + t),
+// routes with ids outside [0, num_rows) skipped; H a multiple of 8.  The rows of
+// eight routes are read before the first is added.
 __global__ void __launch_bounds__(kCombineThreads) combine_routes_kernel(const uint16_t* __restrict__ routes,
                                                                          const int32_t* __restrict__ ids, int num_rows,
-                                                                         const float* __restrict__ shared, int M, int k,
-                                                                         int H, uint16_t* __restrict__ y) {
+                                                                         int shared, int M, int k, int H,
+                                                                         uint16_t* __restrict__ y) {
   const long long i = static_cast<long long>(blockIdx.x) * kCombineThreads + threadIdx.x;
   const int per = H / 8;
   if (i >= static_cast<long long>(M) * per) return;
@@ -54,8 +54,12 @@ __global__ void __launch_bounds__(kCombineThreads) combine_routes_kernel(const u
     }
   }
   if (shared) {
+    const u32x4 v = *reinterpret_cast<const u32x4*>(routes + (static_cast<size_t>(M) * k + t) * H + h);
 #pragma unroll
-    for (int w = 0; w < 8; ++w) acc[w] += shared[static_cast<size_t>(t) * H + h + w];
+    for (int w = 0; w < 4; ++w) {
+      acc[2 * w] += __uint_as_float(v[w] << 16);
+      acc[2 * w + 1] += __uint_as_float(v[w] & 0xffff0000u);
+    }
   }
   u32x4 o;
 #pragma unroll
@@ -116,11 +120,11 @@ hipError_t launch_matmul(const MatmulArgs& a, hipStream_t stream) {
   return launch_matmul_tile(a, best->shape, best->shape == kTile256x128 && a.E > 1 && rows <= 64ll * a.E, stream);
 }
 
-hipError_t launch_combine_routes(const uint16_t* routes, const int32_t* ids, int num_rows, const float* shared, int M,
+hipError_t launch_combine_routes(const uint16_t* routes, const int32_t* ids, int num_rows, bool shared, int M,
                                  int k, int H, uint16_t* y, hipStream_t stream) {
   const long long n = static_cast<long long>(M) * (H / 8);
   hipLaunchKernelGGL(combine_routes_kernel, dim3(static_cast<unsigned>((n + kCombineThreads - 1) / kCombineThreads)), dim3(kCombineThreads), 0, stream, routes,
-                     ids, num_rows, shared, M, k, H, y);
+                     ids, num_rows, static_cast<int>(shared), M, k, H, y);
   return hipGetLastError();
 }
 

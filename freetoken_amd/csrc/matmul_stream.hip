@@ -29,9 +29,10 @@ __device__ __forceinline__ bool find_block(const MatmulArgs& a, int block, int b
   }
   const int lane = lane_id();
   int done = 0;
-  for (int e0 = 0; e0 < a.E; e0 += kWave) {
+  const int groups = group_count(a);
+  for (int e0 = 0; e0 < groups; e0 += kWave) {
     int lo = 0, hi = 0;
-    if (e0 + lane < a.E) group_range(a, e0 + lane, lo, hi);
+    if (e0 + lane < groups) group_range(a, e0 + lane, lo, hi);
     const int nb = (hi - lo + block - 1) / block;
     int sum = nb;
 #pragma unroll
@@ -71,6 +72,12 @@ __global__ void __launch_bounds__(W* kWave) matmul_stream_kernel(MatmulArgs a) {
   const int n0 = (blockIdx.x * kGroups + wave / KS) * 16 * NJ;
   const uint32_t rb = static_cast<uint32_t>(a.K) * (INT8 ? 1 : 2);
 
+  const bool extra = e == a.E;
+  const uint8_t* const w = extra ? a.extra_w : a.w + static_cast<size_t>(e) * a.N * rb;
+  const float* const ws = extra ? a.extra_ws : a.ws + static_cast<size_t>(e) * a.N;
+  const float limit = extra ? a.extra_limit : a.limit;
+  auto x_row = [&](int r) -> uint32_t { return r < a.rows ? r / a.top_k : r - a.rows + a.extra_x; };
+
   // rows of y and of x in this lane's columns
   int route[CT];
   uint32_t xvoff[CT];
@@ -79,15 +86,15 @@ __global__ void __launch_bounds__(W* kWave) matmul_stream_kernel(MatmulArgs a) {
     const int i = begin + 16 * c + r16;
     int r = -1;
     if (i < end) {
-      r = a.order ? a.order[i] : i;
-      if (static_cast<uint32_t>(r) >= static_cast<uint32_t>(a.rows)) r = -1;
+      r = a.order && !extra ? a.order[i] : i;
+      if (static_cast<uint32_t>(r) >= static_cast<uint32_t>(a.rows + a.extra)) r = -1;
     }
     route[c] = r;
-    xvoff[c] = r < 0 ? kOutOfRange : static_cast<uint32_t>(r / a.top_k) * rb + 16 * g;
+    xvoff[c] = r < 0 ? kOutOfRange : x_row(r) * rb + 16 * g;
   }
   // weights: lane l of copy h of a tile takes chunk (l % 8) ^ (l / 8) of row 8h + l / 8
   const int q = (lane & 7) ^ (lane >> 3);
-  const uint8_t* wexp = a.w + (static_cast<size_t>(e) * a.N + n0) * rb;
+  const uint8_t* wexp = w + static_cast<size_t>(n0) * rb;
   const __amdgpu_buffer_rsrc_t rw =
       make_rsrc(wexp, static_cast<uint32_t>(max(GATE ? a.N - n0 : min(a.N - n0, 16 * RT), 0)) * rb);
   const __amdgpu_buffer_rsrc_t rx = make_rsrc(a.x, static_cast<uint32_t>(a.x_rows) * rb);
@@ -182,18 +189,18 @@ __global__ void __launch_bounds__(W* kWave) matmul_stream_kernel(MatmulArgs a) {
       if (r < 0 || nn >= n_out) continue;
       const acc_t sg = sum(j, c);
       const acc_t su = GATE ? sum(NJ + j, c) : sg;
-      const float xs = INT8 ? a.xs[r / a.top_k] : 1.0f;
-      const float wt = a.row_weight ? a.row_weight[r] : 1.0f;
+      const float xs = INT8 ? a.xs[x_row(r)] : 1.0f;
+      const float wt = a.row_weight && r < a.rows ? a.row_weight[r] : 1.0f;
       float o[4];
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         const int f = min(nn + v, n_out - 1);
         float y = static_cast<float>(sg[v]);
-        if (INT8) y *= a.ws[static_cast<size_t>(e) * a.N + f] * xs;
+        if (INT8) y *= ws[f] * xs;
         if constexpr (GATE) {
           float u = static_cast<float>(su[v]);
-          if (INT8) u *= a.ws[static_cast<size_t>(e) * a.N + n_out + f] * xs;
-          swiglu_clamp(a.limit, y, u);
+          if (INT8) u *= ws[n_out + f] * xs;
+          swiglu_clamp(limit, y, u);
           y = act_apply(a.act, y) * u;
         }
         o[v] = y * wt;
@@ -220,7 +227,8 @@ template <bool INT8, bool GATE, int RT, int CT, int S, int KS, int W>
 hipError_t launch_one(const MatmulArgs& a, hipStream_t stream) {
   constexpr auto kernel = matmul_stream_kernel<INT8, GATE, RT, CT, S, KS, W>;
   const int n_out = GATE ? a.N / 2 : a.N, feats = 16 * (GATE ? RT / 2 : RT) * (W / KS);
-  const long long blocks = std::min<long long>(a.rows, a.rows / (16 * CT) + a.E);
+  const long long blocks =
+      std::min<long long>(a.rows, a.rows / (16 * CT) + a.E) + (a.extra + 16 * CT - 1) / (16 * CT);
   hipLaunchKernelGGL(kernel, dim3((n_out + feats - 1) / feats, static_cast<unsigned>(blocks)),
                      dim3(W * kWave), 0, stream, a);
   return hipGetLastError();

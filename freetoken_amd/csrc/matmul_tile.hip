@@ -34,7 +34,7 @@ struct TileLds {
   // per tile parity: the tile's rows of y, their scales and weights, and the channel scales
   static constexpr int kSide = (3 * COLS + ROWS) * 4;
   static constexpr int kFixed = kRing + 2 * kSide;
-  static int bytes(int E) { return kFixed + 2 * (E + 1) * static_cast<int>(sizeof(int)); }
+  static int bytes(int groups) { return kFixed + 2 * (groups + 1) * static_cast<int>(sizeof(int)); }
 };
 
 template <bool INT8, bool GATE, int WR, int WC, int RT, int CT, int S, bool NT>
@@ -45,9 +45,9 @@ __global__ void __launch_bounds__(kWave* WR* WC) matmul_tile_kernel(MatmulArgs a
   constexpr int D = S - 1;  // prefetch distance in K steps
   constexpr int kChunk = 2048 / COLS;  // M blocks that sweep the N tiles together
   extern __shared__ __attribute__((aligned(16))) uint8_t t_lds[];
-  int* const s_blk = reinterpret_cast<int*>(t_lds + L::kFixed);  // [E + 1] first block of every group
-  const int E = a.E;
-  int* const s_beg = s_blk + E + 1;                              // [E + 1] first row of every group
+  const int E = a.E, G = group_count(a);
+  int* const s_blk = reinterpret_cast<int*>(t_lds + L::kFixed);  // [G + 1] first block of every group
+  int* const s_beg = s_blk + G + 1;                              // [E + 1] first row of every group, the last one's end
   const auto s_route = [&](int b) { return reinterpret_cast<int*>(t_lds + L::kRing + b * L::kSide); };
   const auto s_xs = [&](int b) { return reinterpret_cast<float*>(t_lds + L::kRing + b * L::kSide) + COLS; };
   const auto s_rw = [&](int b) { return reinterpret_cast<float*>(t_lds + L::kRing + b * L::kSide) + 2 * COLS; };
@@ -66,9 +66,9 @@ __global__ void __launch_bounds__(kWave* WR* WC) matmul_tile_kernel(MatmulArgs a
   // ---- blocks of every group
   if (wave == 0) {
     int done = 0;
-    for (int e0 = 0; e0 <= E; e0 += kWave) {
+    for (int e0 = 0; e0 <= G; e0 += kWave) {
       int lo = 0, hi = 0;
-      if (e0 + lane < E) group_range(a, e0 + lane, lo, hi);
+      if (e0 + lane < G) group_range(a, e0 + lane, lo, hi);
       const int nb = (hi - lo + COLS - 1) / COLS;
       int sum = nb;
 #pragma unroll
@@ -76,10 +76,8 @@ __global__ void __launch_bounds__(kWave* WR* WC) matmul_tile_kernel(MatmulArgs a
         const int y = __shfl_up(sum, off, kWave);
         if (lane >= off) sum += y;
       }
-      if (e0 + lane <= E) {
-        s_blk[e0 + lane] = done + sum - nb;
-        s_beg[e0 + lane] = lo;
-      }
+      if (e0 + lane <= G) s_blk[e0 + lane] = done + sum - nb;
+      if (e0 + lane < E) s_beg[e0 + lane] = lo;
       done += __shfl(sum, kWave - 1, kWave);
     }
     if (lane == 0) s_beg[E] = a.offsets ? min(max(a.offsets[E], 0), a.rows) : a.rows;
@@ -87,21 +85,23 @@ __global__ void __launch_bounds__(kWave* WR* WC) matmul_tile_kernel(MatmulArgs a
   __syncthreads();
 
   const auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-  const int total = uniform(s_blk[E]) * ntiles;
+  const int total = uniform(s_blk[G]) * ntiles;
   auto map_tile = [&](int b, MTile& t) -> bool {
     if (b >= total) return false;
     const int wg = xcd_major(b, total);
     int owner = 0;
-    if (E > 1) {  // the largest group whose first tile is <= wg
+    if (G > 1) {  // the largest group whose first tile is <= wg
       owner = -1;
       const int l = fresh_lane();
-      for (int e0 = 0; e0 < E; e0 += kWave)
-        owner += __popcll(__ballot(e0 + l < E && s_blk[min(e0 + l, E)] * ntiles <= wg));
+      for (int e0 = 0; e0 < G; e0 += kWave)
+        owner += __popcll(__ballot(e0 + l < G && s_blk[min(e0 + l, G)] * ntiles <= wg));
       owner = uniform(owner);
     }
     const int b0 = uniform(s_blk[owner]), nb = uniform(s_blk[owner + 1]) - b0;
     const MNTile mn = chunked<kChunk>(wg - b0 * ntiles, nb, ntiles);
-    const int beg = uniform(s_beg[owner]), end = max(beg, uniform(s_beg[owner + 1]));
+    const bool extra = owner == E;
+    const int beg = extra ? a.rows : uniform(s_beg[owner]);
+    const int end = extra ? a.rows + a.extra : max(beg, uniform(s_beg[min(owner, E - 1) + 1]));
     t.e = owner;
     t.begin = beg + mn.m * COLS;
     t.end = min(end, t.begin + COLS);
@@ -133,7 +133,9 @@ __global__ void __launch_bounds__(kWave* WR* WC) matmul_tile_kernel(MatmulArgs a
   const uint32_t magic = a.top_k == 1 ? 0u : static_cast<uint32_t>(((uint64_t{1} << 32) + a.top_k - 1) / a.top_k);
   auto x_row = [&](int r) -> uint32_t {
     uint32_t q = static_cast<uint32_t>(r);
-    if (magic) {
+    if (r >= a.rows) {
+      q += a.extra_x - a.rows;
+    } else if (magic) {
       q = __umulhi(q, magic);
       // the rounded-up reciprocal gives at most one too many
       q -= q * static_cast<uint32_t>(a.top_k) > static_cast<uint32_t>(r) ? 1u : 0u;
@@ -143,12 +145,12 @@ __global__ void __launch_bounds__(kWave* WR* WC) matmul_tile_kernel(MatmulArgs a
   // row of y in column col of tile t, or -1
   auto route_of = [&](const MTile& t, int b, int col) -> int {
     const int r = s_route(b)[col];
-    return t.begin + col < t.end && static_cast<uint32_t>(r) < static_cast<uint32_t>(a.rows) ? r : -1;
+    return t.begin + col < t.end && static_cast<uint32_t>(r) < static_cast<uint32_t>(a.rows + a.extra) ? r : -1;
   };
   auto fetch_routes = [&](const MTile& t, int b) {  // wave w: columns [64 w, 64 w + 64)
     if (64 * wave >= COLS) return;
     const int ln = fresh_lane();
-    if (a.order)
+    if (a.order && t.e != E)
       lds_buf4(make_rsrc(a.order + t.begin, static_cast<uint32_t>(t.end - t.begin) * 4),
                reinterpret_cast<uint8_t*>(s_route(b) + 64 * wave), (64 * wave + ln) * 4, 0);
     else
@@ -156,8 +158,9 @@ __global__ void __launch_bounds__(kWave* WR* WC) matmul_tile_kernel(MatmulArgs a
   };
   auto setup = [&](const MTile& t, int b) {
     const int n0 = n0_of(t);
-    wbase = uniform_u64(reinterpret_cast<uint64_t>(a.w) +
-                        (static_cast<uint64_t>(t.e) * static_cast<uint32_t>(a.N) + static_cast<uint32_t>(n0)) * rb);
+    const bool extra = t.e == E;
+    const uint64_t first = (extra ? 0 : static_cast<uint64_t>(t.e) * static_cast<uint32_t>(a.N)) + static_cast<uint32_t>(n0);
+    wbase = uniform_u64(reinterpret_cast<uint64_t>(extra ? a.extra_w : a.w) + first * rb);
     wrange = uniform(static_cast<int>(static_cast<uint32_t>(GATE ? a.N - n0 : min(a.N - n0, ROWS)) * rb));
     const int ln = fresh_lane();
 #pragma unroll
@@ -170,10 +173,10 @@ __global__ void __launch_bounds__(kWave* WR* WC) matmul_tile_kernel(MatmulArgs a
       if (INT8)
         lds_buf4(rsrc_xs, reinterpret_cast<uint8_t*>(s_xs(b) + 64 * wave), r < 0 ? kOutOfRange : x_row(r) * 4, 0);
       if (a.row_weight)  // (rows < 2^31: 64-bit addresses through the descriptor's base would not reach past 2 GiB)
-        s_rw(b)[64 * wave + ln] = r < 0 ? 0.f : a.row_weight[r];
+        s_rw(b)[64 * wave + ln] = r < 0 ? 0.f : r < a.rows ? a.row_weight[r] : 1.0f;
     }
     if (INT8 && 64 * wave < ROWS) {
-      const uint64_t ws = uniform_u64(reinterpret_cast<uint64_t>(a.ws) + (static_cast<uint64_t>(t.e) * a.N + n0) * 4);
+      const uint64_t ws = uniform_u64(reinterpret_cast<uint64_t>(extra ? a.extra_ws : a.ws) + first * 4);
       lds_buf4(make_rsrc(reinterpret_cast<const void*>(ws), uniform((a.N - n0) * 4)),
                reinterpret_cast<uint8_t*>(s_ws(b) + 64 * wave), static_cast<uint32_t>(trow_rel(64 * wave + ln)) * 4, 0);
     }
@@ -244,6 +247,7 @@ __global__ void __launch_bounds__(kWave* WR* WC) matmul_tile_kernel(MatmulArgs a
     uint8_t* const mine = stg + wave * (32 * RB);
     static_assert(WR * WC * 32 * RB <= L::kStage, "the staging areas fit a stage");
     const bool whole = n_out % 8 == 0;
+    const float limit = t.e == E ? a.extra_limit : a.limit;
     const float* const wsp = s_ws(b) + 32 * RT * wr + 4 * half;
 #pragma unroll
     for (int i = 0; i < CT; ++i) {
@@ -265,7 +269,7 @@ __global__ void __launch_bounds__(kWave* WR* WC) matmul_tile_kernel(MatmulArgs a
             if constexpr (GATE) {
               float u = static_cast<float>(acc[RT / 2 + j][i][4 * q + v]);
               if (INT8) u *= wu[v] * xs;
-              swiglu_clamp(a.limit, y, u);
+              swiglu_clamp(limit, y, u);
               y = act_apply(a.act, y) * u;
             }
             o[v] = y * rw;
@@ -382,7 +386,7 @@ hipError_t launch_tile(const MatmulArgs& a, hipStream_t stream) {
   constexpr int ROWS = 32 * RT * WR, COLS = 32 * CT * WC;
   constexpr auto kernel = matmul_tile_kernel<INT8, GATE, WR, WC, RT, CT, S, NT>;
   using L = TileLds<ROWS, COLS, WR * WC, S>;
-  const int lds = L::bytes(a.E);
+  const int lds = L::bytes(group_count(a));
   // once on every device
   int dev = 0;
   hipError_t err = hipGetDevice(&dev);
@@ -395,7 +399,8 @@ hipError_t launch_tile(const MatmulArgs& a, hipStream_t stream) {
     if (dev <= 63) ready |= uint64_t{1} << dev;
   }
   const int n_out = GATE ? a.N / 2 : a.N, out_rows = GATE ? ROWS / 2 : ROWS;
-  const long long blocks = std::min<long long>(a.rows, static_cast<long long>(a.rows) / COLS + a.E);
+  const long long blocks =
+      std::min<long long>(a.rows, static_cast<long long>(a.rows) / COLS + a.E) + (a.extra + COLS - 1) / COLS;
   const long long tiles = blocks * ((n_out + out_rows - 1) / out_rows);
   const int per_cu = std::max(1, 160 * 1024 / lds);
   const int wgs = static_cast<int>(std::min<long long>(tiles, 256ll * per_cu));

@@ -385,9 +385,9 @@ int ftmoe_grouped_matmul(const ftmoe_grouped* args, ftmoe_stream_t stream);
 /* Expert layer of an INT8 bank for a precomputed routing, decode and prefill
  * alike: tokens are quantised (ftmoe_act_quant_int8), multiplied with the gate
  * and up rows, act(gate) * up is rounded to bf16 and quantised per route,
- * multiplied with the down rows and the router weight, and the routes of a token
- * (and the shared expert, nullable, an INT8 bank of one row) are summed in
- * float32.  Ids outside [0, num_rows) are skipped.  num_rows <= 1023. */
+ * multiplied with the down rows and the router weight to a bf16 row, and a token's
+ * rows (the last one the shared expert's: nullable, an INT8 bank of one row) are
+ * summed in float32.  Ids outside [0, num_rows) are skipped.  num_rows <= 1023. */
 size_t ftmoe_experts_int8_workspace(int M, int top_k, const ftmoe_bank* bank, const ftmoe_bank* shared);
 int ftmoe_experts_int8(const void* x, int M, int top_k, const float* topk_w, const int32_t* topk_ids,
                        const ftmoe_bank* bank, const ftmoe_bank* shared, int activation, void* y, void* workspace,

@@ -404,8 +404,9 @@ def values(x):
     return torch.where(a > 0, (127 * x / torch.where(a > 0, a, 1.0)).round() * (a / 127), 0.0)
 
 
-def layer_ref(x, tw, ids, bank, shared, act, limit=0.0):
+def layer_ref(x, tw, ids, bank, shared, act):
     def mlp(rows, b, e):
+        limit = b.swiglu_limit
         h = rows @ (b.gate_up[e].double() * b.gate_up_scale[e].double()[:, None]).T
         gate, up = h.chunk(2, dim=1)
         if limit > 0:
@@ -428,6 +429,7 @@ LAYER = [  # M, k, E, H, I, shared inter, activation, limit
     (7, 8, 128, 336, 112, 48, "silu", 0.0),
     (64, 8, 64, 512, 256, 256, "gelu", 0.0),
     (130, 4, 8, 272, 400, 16, "silu", 0.75),
+    (40, 2, 24, 272, 144, 144, "silu", 0.75),
     (700, 6, 32, 640, 384, 384, "gelu_tanh", 0.0),
     (1500, 8, 16, 512, 256, 0, "silu", 0.0),
 ]
@@ -442,13 +444,13 @@ def test_experts_int8(dev, case):
     shared = make_bank(dev, g, 1, H, Is) if Is else None
     bank.swiglu_limit = limit
     if shared:
-        shared.swiglu_limit = limit
+        shared.swiglu_limit = 2 * limit
     tw, ids = routing(dev, g, M, k, E)
     if M > 2:  # padded places: no expert
         ids[M // 2 :: 3] = -1
         ids[0, 0] = E
     y = ops.experts_int8(x, tw, ids, bank, shared=shared, activation=act)
-    ref = layer_ref(x, tw, ids, bank, shared, act, limit)
+    ref = layer_ref(x, tw, ids, bank, shared, act)
     got, want = y.double().cpu().numpy(), ref.cpu().numpy()
     assert max_rel(got, want) <= MAX_REL_TOL and cosine(got, want) >= COS_TOL, (max_rel(got, want), cosine(got, want))
     if shared is None and M > 2:
@@ -457,10 +459,7 @@ def test_experts_int8(dev, case):
     q, s = ops.act_quant_int8(x)
     order, offsets = ops.group_routes(ids, E)
 
-    def clamped(b):  # the clamp is the layer's own: the products alone have none
-        return limit == 0
-
-    if not clamped(bank):
+    if limit:  # the clamp is the layer's own: the products alone have none
         return
     h = torch.zeros((M * k, I), dtype=torch.bfloat16, device=dev)
     ops.grouped_matmul(q, bank.gate_up, offsets, order=order, top_k=k, x_scale=s, w_scale=bank.gate_up_scale,
@@ -474,7 +473,7 @@ def test_experts_int8(dev, case):
         total = total + o.view(M, k, H)[:, j].float()
     if shared is not None:
         sq, ss = ops.act_quant_int8(ops.matmul_int8(q, s, shared.gate_up[0], shared.gate_up_scale[0], activation=act))
-        total = total + ops.matmul_int8(sq, ss, shared.down[0], shared.down_scale[0], out_dtype=torch.float32)
+        total = total + ops.matmul_int8(sq, ss, shared.down[0], shared.down_scale[0]).float()
     assert torch.equal(y, total.to(torch.bfloat16))
 
 
