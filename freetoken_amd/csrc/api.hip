@@ -1089,7 +1089,11 @@ int ftmoe_experts_int8(const void* x, int M, int top_k, const float* topk_w, con
   if (!run(ftmoe::launch_group_routes(g, L.hist, stream), "experts_int8 grouping and x quant")) return rc;
   if (!run(ftmoe::launch_matmul(up, stream), "experts_int8 gate_up")) return rc;
   // (rows of skipped routes hold what the workspace held: quantised, never multiplied)
-  if (!run(ftmoe::launch_act_quant_int8(L.act, numel + (joined ? M : 0), bank->inter, L.actq, L.as, stream),
+  if (ftmoe::launch_matmul_quantises(down)) {
+    down.quantise = 1;
+    down.x = reinterpret_cast<const uint8_t*>(L.act);
+    down.xs = nullptr;
+  } else if (!run(ftmoe::launch_act_quant_int8(L.act, numel + (joined ? M : 0), bank->inter, L.actq, L.as, stream),
            "experts_int8 act quant"))
     return rc;
   if (!run(ftmoe::launch_matmul(down, stream), "experts_int8 down")) return rc;

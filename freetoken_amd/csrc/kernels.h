@@ -297,10 +297,13 @@ struct MatmulArgs {
   const uint8_t* extra_w;
   const float* extra_ws;
   float extra_limit;
+  int quantise;             // int8: x is bf16 and quantised on the way (launch_matmul_quantises)
   int out_f32;              // y float32 instead of bf16
   void* y;                  // [rows + extra, N] (N/2 with act)
 };
 hipError_t launch_matmul(const MatmulArgs& a, hipStream_t stream);
+// Whether the product (int8, without act) takes bf16 rows of x as they are.
+bool launch_matmul_quantises(const MatmulArgs& a);
 hipError_t launch_act_quant_int8(const uint16_t* x, int rows, int K, int8_t* q, float* scales, hipStream_t stream);
 // Routes by expert (group.hip), and beside it the quantisation of the tokens where x is given.
 struct GroupArgs {

@@ -64,8 +64,9 @@ __device__ __forceinline__ void group_range(const MatmulArgs& a, int e, int& beg
 
 __host__ __device__ inline int group_count(const MatmulArgs& a) { return a.E + (a.extra > 0 ? 1 : 0); }
 
-// The streaming form, for few rows per group (matmul_stream.hip); wide: 32 features x 32 rows per workgroup, else
-// 16 x 16.
+// The streaming form, for few rows per group (matmul_stream.hip); wide: 32 features x 32 rows per workgroup (16 where x
+// is quantised on the way), else 16 x 16.
+constexpr int kStreamQuantMaxK = 2048;
 hipError_t launch_matmul_stream(const MatmulArgs& a, bool wide, hipStream_t stream);
 
 // The tiled form, for many rows per group (matmul_tile.hip): weight rows x rows of x of a workgroup; once: the weights

@@ -77,17 +77,34 @@ __global__ void __launch_bounds__(kCombineThreads) combine_routes_kernel(const u
 //   8 rows over 128 experts, N 1536 (gate and up), K 2048: 9.1 / 9.9 / 14;
 //   bf16 32 rows over 128, N 1536 (gate and up), K 2048: 28 / 32 / 40; 100 rows over 256: 60 / 51 / 47;
 //   512 rows over 64, N 7168, K 2048: 209 / 158 / 147.
-hipError_t launch_matmul(const MatmulArgs& a, hipStream_t stream) {
+namespace {
+
+enum class Form { kTiles, kStream16, kStream32 };
+
+Form form_of(const MatmulArgs& a) {
   const long long n_out = a.act < 0 ? a.N : a.N / 2, rows = a.rows;
-  const long long row_bytes = static_cast<long long>(a.K) * (a.int8 ? 1 : 2);
   if (rows <= 16ll * a.E) {
     // the small workgroups win while they do not fill the chip, longer where their streams are long
+    const long long row_bytes = static_cast<long long>(a.K) * (a.int8 ? 1 : 2);
     const long long units = (n_out + 15) / 16 * std::min<long long>(rows, (rows + 15) / 16 + a.E - 1);
-    if (units <= 384 || (units <= 1536 && row_bytes >= 4096)) return launch_matmul_stream(a, false, stream);
-    if (units <= 1536) return launch_matmul_stream(a, true, stream);
+    if (units <= 384 || (units <= 1536 && row_bytes >= 4096)) return Form::kStream16;
+    if (units <= 1536) return Form::kStream32;
   } else if (a.E == 1 && rows <= 64) {
-    return launch_matmul_stream(a, true, stream);
+    return Form::kStream32;
   }
+  return Form::kTiles;
+}
+
+}  // namespace
+
+bool launch_matmul_quantises(const MatmulArgs& a) {
+  return a.int8 && a.act < 0 && a.K <= kStreamQuantMaxK && form_of(a) != Form::kTiles;
+}
+
+hipError_t launch_matmul(const MatmulArgs& a, hipStream_t stream) {
+  const Form form = form_of(a);
+  if (form != Form::kTiles) return launch_matmul_stream(a, form == Form::kStream32, stream);
+  const long long n_out = a.act < 0 ? a.N : a.N / 2, rows = a.rows;
   // Tiles: the time of a shape goes by its rounds over the workgroups that fit the
   // chip at once (the mean of the whole rounds and the fraction) times what a round
   // of it takes, from the rates that large calls reach (dense 8192 x 4096 x 7168: 2320, 2140 and

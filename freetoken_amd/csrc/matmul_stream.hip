@@ -6,11 +6,16 @@
 // wave copies its weight lines global -> LDS by LDS-DMA into a ring of its own (no
 // barrier in the K loop): an instruction covers 8 whole 128-byte lines, where a
 // register load in the operand layout covers half lines.  x comes straight to registers.
+//
+// QX: x is bf16.  The workgroup quantises its rows (quant_int8.h, the codes that
+// act_quant_int8 gives) into LDS while its first weights are on their way, which saves
+// a step of one or a few tokens the launch between an expert's two products.
 #include <algorithm>
 
 #include "kernels.h"
 #include "lds_ring.h"
 #include "matmul.h"
+#include "quant_int8.h"
 
 namespace ftmoe {
 
@@ -54,14 +59,18 @@ __device__ __forceinline__ bool find_block(const MatmulArgs& a, int block, int b
   return false;
 }
 
-template <bool INT8, bool GATE, int RT, int CT, int S, int KS, int W>
+template <bool INT8, bool GATE, bool QX, int RT, int CT, int S, int KS, int W>
 __global__ void __launch_bounds__(W* kWave) matmul_stream_kernel(MatmulArgs a) {
   using acc_t = typename Acc<INT8>::type;
   constexpr int kStage = RT * kTile, kRing = S * kStage;
   constexpr int kGroups = W / KS;  // waves that own rows of their own
   constexpr int kRed = KS > 1 ? W * RT * CT * kWave * 16 : 0;
-  constexpr int kPerStep = 2 * RT + 2 * CT;  // vector memory instructions of a step
-  __shared__ __attribute__((aligned(16))) uint8_t lds[std::max(W * kRing, kRed)];
+  constexpr int kPerStep = 2 * RT + (QX ? 0 : 2 * CT);  // vector memory instructions of a step
+  // the quantised rows, their scales
+  constexpr int kXRow = kStreamQuantMaxK + 16, kXRows = QX ? 16 * CT * kXRow : 0;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[std::max(W * kRing, kRed) + kXRows + (QX ? 16 * CT * 4 : 0)];
+  uint8_t* const xq = lds + std::max(W * kRing, kRed);
+  float* const s_xs = reinterpret_cast<float*>(xq + kXRows);
   const int lane = lane_id(), r16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   int e, begin, end;
@@ -113,6 +122,24 @@ __global__ void __launch_bounds__(W* kWave) matmul_stream_kernel(MatmulArgs a) {
 
   uint8_t* const ring = lds + wave * kRing;
   u32x4 xf[S][CT][2];
+  // QX: row k of the workgroup's columns belongs to wave k % W, lane l holding its pieces l, l + 64, ...
+  constexpr int kMine = QX ? 16 * CT / W : 1, kPieces = QX ? kStreamQuantMaxK / 8 / kWave : 1;
+  u32x4 raw[kMine][kPieces];
+  int mine[kMine];
+  if constexpr (QX) {
+#pragma unroll
+    for (int m = 0; m < kMine; ++m) {
+      const int k = m * W + wave, c = m * W / 16;  // (W divides 16: a constant column tile)
+      mine[m] = __builtin_amdgcn_readlane(route[c], k & 15);
+      const u32x4* row = reinterpret_cast<const u32x4*>(a.x + static_cast<size_t>(x_row(max(mine[m], 0))) * rb * 2);
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p) {
+        const int at = lane + p * kWave;
+        raw[m][p] = mine[m] >= 0 && at < a.K / 8 ? row[at] : u32x4{0u, 0u, 0u, 0u};
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
   auto issue = [&](int s, int slot) {  // step s of this wave; past its end: the same instructions, reading zeros
     const uint32_t off = s < n ? 0u : kOutOfRange;
     const bool last = lo + s == nst - 1;
@@ -122,6 +149,7 @@ __global__ void __launch_bounds__(W* kWave) matmul_stream_kernel(MatmulArgs a) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         lds_buf16_nt(rw, ring + slot * kStage + j * kTile + h * 1024, wvoff[j][h] | off | (last ? wdead : 0u), so);
+    if constexpr (!QX)
 #pragma unroll
     for (int c = 0; c < CT; ++c)
 #pragma unroll
@@ -132,7 +160,14 @@ __global__ void __launch_bounds__(W* kWave) matmul_stream_kernel(MatmulArgs a) {
   for (int j = 0; j < RT; ++j)
 #pragma unroll
     for (int c = 0; c < CT; ++c) acc[j][c] = acc_t{};
-  auto compute = [&](int slot) {
+  auto compute = [&](int slot, int s) {
+    if constexpr (QX) {  // (steps past the end, and past K in the last one, meet zero weights)
+      const uint8_t* const at = xq + r16 * kXRow + min(lo + s, nst - 1) * 128 + 16 * g;
+#pragma unroll
+      for (int c = 0; c < CT; ++c)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) xf[slot][c][p] = *reinterpret_cast<const u32x4*>(at + c * 16 * kXRow + 64 * p);
+    }
 #pragma unroll
     for (int j = 0; j < RT; ++j) {
       const uint8_t* row = ring + slot * kStage + j * kTile + r16 * 128;
@@ -149,6 +184,26 @@ __global__ void __launch_bounds__(W* kWave) matmul_stream_kernel(MatmulArgs a) {
     issue(s, s);
     __builtin_amdgcn_sched_barrier(0);
   }
+  if constexpr (QX) {
+#pragma unroll
+    for (int m = 0; m < kMine; ++m) {
+      if (mine[m] < 0) continue;
+      const int k = m * W + wave;
+      uint32_t top = 0;
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p)
+#pragma unroll
+        for (int w4 = 0; w4 < 4; ++w4) top = max_pair(top, raw[m][p][w4]);
+      const RowCodes rc = row_codes(wave_max_pair(top));
+      if (lane == 0) s_xs[k] = rc.scale;
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p)
+        if (lane + p * kWave < a.K / 8)
+          *reinterpret_cast<uint2*>(xq + k * kXRow + 8 * (lane + p * kWave)) = rc.codes(raw[m][p]);
+    }
+    wait_lgkm0();
+    bare_barrier();
+  }
   for (int i = 0; i < n; i += S) {
 #pragma unroll
     for (int s = 0; s < S; ++s) {
@@ -156,7 +211,7 @@ __global__ void __launch_bounds__(W* kWave) matmul_stream_kernel(MatmulArgs a) {
       issue(i + s + S - 1, (s + S - 1) % S);
       wait_vm<(S - 1) * kPerStep>();
       __builtin_amdgcn_sched_barrier(0);
-      compute(s);
+      compute(s, i + s);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -189,7 +244,7 @@ __global__ void __launch_bounds__(W* kWave) matmul_stream_kernel(MatmulArgs a) {
       if (r < 0 || nn >= n_out) continue;
       const acc_t sg = sum(j, c);
       const acc_t su = GATE ? sum(NJ + j, c) : sg;
-      const float xs = INT8 ? a.xs[x_row(r)] : 1.0f;
+      const float xs = QX ? s_xs[16 * c + r16] : INT8 ? a.xs[x_row(r)] : 1.0f;
       const float wt = a.row_weight && r < a.rows ? a.row_weight[r] : 1.0f;
       float o[4];
 #pragma unroll
@@ -223,9 +278,9 @@ __global__ void __launch_bounds__(W* kWave) matmul_stream_kernel(MatmulArgs a) {
   }
 }
 
-template <bool INT8, bool GATE, int RT, int CT, int S, int KS, int W>
+template <bool INT8, bool GATE, bool QX, int RT, int CT, int S, int KS, int W>
 hipError_t launch_one(const MatmulArgs& a, hipStream_t stream) {
-  constexpr auto kernel = matmul_stream_kernel<INT8, GATE, RT, CT, S, KS, W>;
+  constexpr auto kernel = matmul_stream_kernel<INT8, GATE, QX, RT, CT, S, KS, W>;
   const int n_out = GATE ? a.N / 2 : a.N, feats = 16 * (GATE ? RT / 2 : RT) * (W / KS);
   const long long blocks =
       std::min<long long>(a.rows, a.rows / (16 * CT) + a.E) + (a.extra + 16 * CT - 1) / (16 * CT);
@@ -238,15 +293,18 @@ hipError_t launch_one(const MatmulArgs& a, hipStream_t stream) {
 template <int NJ, int CT, int S, int KS, int W>
 hipError_t launch_stream(const MatmulArgs& a, hipStream_t stream) {
   if (a.int8)
-    return a.act < 0 ? launch_one<true, false, NJ, CT, S, KS, W>(a, stream)
-                     : launch_one<true, true, 2 * NJ, CT, S, KS, W>(a, stream);
-  return a.act < 0 ? launch_one<false, false, NJ, CT, S, KS, W>(a, stream)
-                   : launch_one<false, true, 2 * NJ, CT, S, KS, W>(a, stream);
+    return a.act < 0 ? launch_one<true, false, false, NJ, CT, S, KS, W>(a, stream)
+                     : launch_one<true, true, false, 2 * NJ, CT, S, KS, W>(a, stream);
+  return a.act < 0 ? launch_one<false, false, false, NJ, CT, S, KS, W>(a, stream)
+                   : launch_one<false, true, false, 2 * NJ, CT, S, KS, W>(a, stream);
 }
 
 }  // namespace
 
 hipError_t launch_matmul_stream(const MatmulArgs& a, bool wide, hipStream_t stream) {
+  if (a.quantise)
+    return wide ? launch_one<true, false, true, 2, 1, 2, 4, 4>(a, stream)
+                : launch_one<true, false, true, 1, 1, 3, 4, 4>(a, stream);
   return wide ? launch_stream<2, 2, 2, 4, 4>(a, stream) : launch_stream<1, 1, 3, 4, 4>(a, stream);
 }
 

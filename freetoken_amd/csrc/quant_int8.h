@@ -73,6 +73,25 @@ __device__ __forceinline__ uint2 codes8(const u32x4& v, const RowScale& s) {
   return uint2{o[0], o[1]};
 }
 
+// Scale and codes of a row from the bits of its largest magnitudes (wave_max_pair).
+struct RowCodes {
+  float scale;
+  bool live;  // the row has codes other than 0
+  RowScale s;
+  __device__ __forceinline__ uint2 codes(const u32x4& v) const { return live ? codes8(v, s) : uint2{0u, 0u}; }
+};
+
+__device__ __forceinline__ RowCodes row_codes(uint32_t pair) {
+  const uint32_t bits = max(pair & 0xffffu, pair >> 16);
+  const bool finite = bits < 0x7f80u;
+  const float amax = __uint_as_float(bits << 16);
+  RowCodes r;
+  r.scale = finite ? __fdiv_rn(amax, 127.0f) : __uint_as_float(0x7fc00000u);
+  r.live = finite && bits != 0;
+  r.s = row_scale(r.live ? amax : 1.0f);
+  return r;
+}
+
 // Quantises row `row` (live: it exists) with WPR waves, thread t of them; a thread
 // holds up to KEEP 16-byte pieces of the row in registers (KEEP 0: any length, read
 // twice, the second time from a cache).  s_max: a word per wave of the workgroup; with
@@ -109,13 +128,9 @@ __device__ __forceinline__ void quant_row(const uint16_t* __restrict__ x, int ro
 #pragma unroll
     for (int w = 0; w < WPR; ++w) m = max_pair(m, s_max[first + w]);
   }
-  const uint32_t bits = max(m & 0xffffu, m >> 16);
-  const bool finite = bits < 0x7f80u, some = bits != 0;
-  const float amax = __uint_as_float(bits << 16);
-  if (live && t == 0) scales[row] = finite ? __fdiv_rn(amax, 127.0f) : __uint_as_float(0x7fc00000u);
-  const bool codes = finite && some;
-  const RowScale s = row_scale(codes ? amax : 1.0f);
-  auto put = [&](int p, const u32x4& u) { qr[p] = codes ? codes8(u, s) : uint2{0u, 0u}; };
+  const RowCodes r = row_codes(m);
+  if (live && t == 0) scales[row] = r.scale;
+  auto put = [&](int p, const u32x4& u) { qr[p] = r.codes(u); };
   if constexpr (KEEP) {
 #pragma unroll
     for (int i = 0; i < KEEP; ++i)
