@@ -64,13 +64,16 @@ __device__ __forceinline__ void group_range(const MatmulArgs& a, int e, int& beg
 
 __host__ __device__ inline int group_count(const MatmulArgs& a) { return a.E + (a.extra > 0 ? 1 : 0); }
 
-// The streaming form, for few rows per group (matmul_stream.hip); wide: 32 features x 32 rows per workgroup (16 where x
-// is quantised on the way), else 16 x 16.
+// The streaming form, for few rows per group (matmul_stream.hip): a workgroup has
+// 16 features x 16 rows with K split over its waves (split), 64 features x 16 rows,
+// each wave with the whole of K (whole), or 32 features x 32 rows, split (wide; not
+// where x is quantised on the way).
+enum StreamShape { kStreamSplit, kStreamWhole, kStreamWide };
 constexpr int kStreamQuantMaxK = 2048;
-hipError_t launch_matmul_stream(const MatmulArgs& a, bool wide, hipStream_t stream);
+hipError_t launch_matmul_stream(const MatmulArgs& a, StreamShape shape, hipStream_t stream);
 
-// The tiled form, for many rows per group (matmul_tile.hip): weight rows x rows of x of a workgroup; once: the weights
-// are read about once, past the caches.
+// The tiled form, for many rows per group (matmul_tile.hip): weight rows x rows of x
+// of a workgroup; once: the weights are read about once, past the caches.
 enum TileShape { kTile128x64, kTile256x128, kTile256x256 };
 hipError_t launch_matmul_tile(const MatmulArgs& a, TileShape shape, bool once, hipStream_t stream);
 

@@ -70,40 +70,47 @@ __global__ void __launch_bounds__(kCombineThreads) combine_routes_kernel(const u
 }  // namespace
 
 // Forms and tiles are chosen from the sizes known on the host: the rows per group
-// are R / E on average.  Measured (us, int8 unless said; stream 16 x 16 / stream 32 x 32 /
-// tiles of 128 x 64 / 256 x 128 / 256 x 256):
-//   one group, N 4096, K 7168: 1 row 7.1 / 9.9 / 22 / 38 / 72, 16 rows 8.4 / 10.6 / 22, 48 rows 19 / 12.6 / 22;
-//   N 7168, K 2048: 16 rows 6.5 / 5.7 / 10, 64 rows - / 9 / 10.5, 128 rows - / 15 / 10.7 / 16;
-//   8 rows over 128 experts, N 1536 (gate and up), K 2048: 9.1 / 9.9 / 14;
-//   bf16 32 rows over 128, N 1536 (gate and up), K 2048: 28 / 32 / 40; 100 rows over 256: 60 / 51 / 47;
-//   512 rows over 64, N 7168, K 2048: 209 / 158 / 147.
+// are R / E on average.  Measured (us, int8 unless said; streams split / whole /
+// wide | tiles of 128 x 64 / 256 x 128):
+//   one group, N 4096, K 7168: 1 row 7.1 / - / 9.9 | 22 / 38, 16 rows 8.4 / - / 10.6 | 22, 48 rows 19 / - / 12.6 | 22;
+//   N 7168, K 2048: 16 rows 6.5 / - / 5.7 | 10, 64 rows - / - / 9 | 10.5, 128 rows - / - / 15 | 10.7 / 16;
+//   128 experts, N 1536 (gate and up), K 2048: 8 rows 9.1 / 10.1 / 9.9 | 14, 64 rows 39 / 30 / 35 | 36, 256 rows 76 /
+//   58 / 69 | 62, 512 rows 82 / 61 / 73 | 64; N 2048, K 768: 64 rows 30 / 17 / 25 | 20, 512 rows 70 / 35 / 52 | 38;
+//   64 experts, N 7168, K 2048, 512 rows 209 / 150 / 158 | 147;
+//   rows of 4 KB and more: bf16 N 1536, K 2048, 64 rows over 128 experts 56 / 68 / 58 | 70; N 4096, K 7168, 9 rows
+//   over 65 43 / 56 / 47 | 57, 300 over 64 270 / 268 / 268 | 273.
 namespace {
 
-enum class Form { kTiles, kStream16, kStream32 };
+enum class Form { kTiles, kSplit, kWhole, kWide };
 
 Form form_of(const MatmulArgs& a) {
-  const long long n_out = a.act < 0 ? a.N : a.N / 2, rows = a.rows;
-  if (rows <= 16ll * a.E) {
-    // the small workgroups win while they do not fill the chip, longer where their streams are long
-    const long long row_bytes = static_cast<long long>(a.K) * (a.int8 ? 1 : 2);
-    const long long units = (n_out + 15) / 16 * std::min<long long>(rows, (rows + 15) / 16 + a.E - 1);
-    if (units <= 384 || (units <= 1536 && row_bytes >= 4096)) return Form::kStream16;
-    if (units <= 1536) return Form::kStream32;
-  } else if (a.E == 1 && rows <= 64) {
-    return Form::kStream32;
-  }
-  return Form::kTiles;
+  const long long n_out = a.act < 0 ? a.N : a.N / 2, rows = a.rows, E = a.E;
+  const long long tiles = (n_out + 15) / 16;  // of 16 features
+  if (E == 1) return rows <= 16 && tiles <= 384 ? Form::kSplit : rows <= 64 ? Form::kWide : Form::kTiles;
+  if (rows > 4 * E) return rows <= 16 * E && tiles * E <= 1536 ? Form::kWide : Form::kTiles;
+  // K is split where there are too few workgroups without it, or rows long enough for four streams
+  const long long row_bytes = static_cast<long long>(a.K) * (a.int8 ? 1 : 2);
+  return row_bytes >= 4096 || tiles * std::min(rows, E) <= 512 ? Form::kSplit : Form::kWhole;
 }
 
 }  // namespace
 
 bool launch_matmul_quantises(const MatmulArgs& a) {
-  return a.int8 && a.act < 0 && a.K <= kStreamQuantMaxK && form_of(a) != Form::kTiles;
+  const Form form = form_of(a);
+  // Saves a launch, but every workgroup quantises its group's rows anew.  An expert layer (us, with / without):
+  // 8 routes over 16 experts (H 1024, I 512) 16.6 / 17.9; over 128 (H 2048, I 768) 8 routes 21.1 / 22.8, 64 routes
+  // 60.7 / 55.2, 512 121 / 106.
+  return a.int8 && a.act < 0 && a.K <= kStreamQuantMaxK && a.rows <= 32 &&
+         (form == Form::kSplit || form == Form::kWhole);
 }
 
 hipError_t launch_matmul(const MatmulArgs& a, hipStream_t stream) {
-  const Form form = form_of(a);
-  if (form != Form::kTiles) return launch_matmul_stream(a, form == Form::kStream32, stream);
+  switch (form_of(a)) {
+    case Form::kSplit: return launch_matmul_stream(a, kStreamSplit, stream);
+    case Form::kWhole: return launch_matmul_stream(a, kStreamWhole, stream);
+    case Form::kWide: return launch_matmul_stream(a, kStreamWide, stream);
+    default: break;
+  }
   const long long n_out = a.act < 0 ? a.N : a.N / 2, rows = a.rows;
   // Tiles: the time of a shape goes by its rounds over the workgroups that fit the
   // chip at once (the mean of the whole rounds and the fraction) times what a round
@@ -140,8 +147,9 @@ hipError_t launch_matmul(const MatmulArgs& a, hipStream_t stream) {
 hipError_t launch_combine_routes(const uint16_t* routes, const int32_t* ids, int num_rows, bool shared, int M,
                                  int k, int H, uint16_t* y, hipStream_t stream) {
   const long long n = static_cast<long long>(M) * (H / 8);
-  hipLaunchKernelGGL(combine_routes_kernel, dim3(static_cast<unsigned>((n + kCombineThreads - 1) / kCombineThreads)), dim3(kCombineThreads), 0, stream, routes,
-                     ids, num_rows, static_cast<int>(shared), M, k, H, y);
+  hipLaunchKernelGGL(combine_routes_kernel,
+                     dim3(static_cast<unsigned>((n + kCombineThreads - 1) / kCombineThreads)), dim3(kCombineThreads), 0,
+                     stream, routes, ids, num_rows, static_cast<int>(shared), M, k, H, y);
   return hipGetLastError();
 }
 

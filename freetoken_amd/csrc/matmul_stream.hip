@@ -1,8 +1,9 @@
 // Streaming form of the matrix products of MatmulArgs, for few rows per group:
 // the time is that of reading the weights once.
 //
-// A workgroup of 4 waves computes 16 RT weight rows x 16 CT rows of x of one group,
-// the waves splitting K and adding their sums through LDS in a fixed order.  Each
+// A workgroup has 4 waves, a wave 16 RT weight rows x 16 CT rows of x of one group.
+// KS waves share the same weight rows and split K between them, adding their sums
+// through LDS in a fixed order; groups of KS waves have weight rows of their own.  Each
 // wave copies its weight lines global -> LDS by LDS-DMA into a ring of its own (no
 // barrier in the K loop): an instruction covers 8 whole 128-byte lines, where a
 // register load in the operand layout covers half lines.  x comes straight to registers.
@@ -301,11 +302,15 @@ hipError_t launch_stream(const MatmulArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-hipError_t launch_matmul_stream(const MatmulArgs& a, bool wide, hipStream_t stream) {
+hipError_t launch_matmul_stream(const MatmulArgs& a, StreamShape shape, hipStream_t stream) {
   if (a.quantise)
-    return wide ? launch_one<true, false, true, 2, 1, 2, 4, 4>(a, stream)
-                : launch_one<true, false, true, 1, 1, 3, 4, 4>(a, stream);
-  return wide ? launch_stream<2, 2, 2, 4, 4>(a, stream) : launch_stream<1, 1, 3, 4, 4>(a, stream);
+    return shape == kStreamWhole ? launch_one<true, false, true, 1, 1, 3, 1, 4>(a, stream)
+                                 : launch_one<true, false, true, 1, 1, 3, 4, 4>(a, stream);
+  switch (shape) {
+    case kStreamSplit: return launch_stream<1, 1, 3, 4, 4>(a, stream);
+    case kStreamWhole: return launch_stream<1, 1, 3, 1, 4>(a, stream);
+    default: return launch_stream<2, 2, 2, 4, 4>(a, stream);
+  }
 }
 
 }  // namespace ftmoe

@@ -7,6 +7,7 @@
 // next S - 1 steps are in flight while a step computes, and the ring runs on from
 // tile to tile (the workgroups are persistent, one walk over the tiles each).
 #include <algorithm>
+#include <atomic>
 
 #include "kernels.h"
 #include "lds_ring.h"
@@ -391,12 +392,12 @@ hipError_t launch_tile(const MatmulArgs& a, hipStream_t stream) {
   int dev = 0;
   hipError_t err = hipGetDevice(&dev);
   if (err != hipSuccess) return err;
-  static uint64_t ready = 0;  // (two threads at once set the same attribute twice)
-  if (dev > 63 || !(ready >> dev & 1)) {
+  static std::atomic<uint64_t> ready{0};  // (two threads at once set the same attribute twice)
+  if (dev > 63 || !(ready.load(std::memory_order_acquire) >> dev & 1)) {
     err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                               160 * 1024);
     if (err != hipSuccess) return err;
-    if (dev <= 63) ready |= uint64_t{1} << dev;
+    if (dev <= 63) ready.fetch_or(uint64_t{1} << dev, std::memory_order_release);
   }
   const int n_out = GATE ? a.N / 2 : a.N, out_rows = GATE ? ROWS / 2 : ROWS;
   const long long blocks =
