@@ -284,7 +284,7 @@ struct MatmulArgs {
   const uint8_t* w;         // [E, N, K]; with act: gate rows [0, N/2), up rows [N/2, N) of every matrix
   const float* ws;          // int8: [E, N] scale of every output channel
   int E, N, K;
-  int rows, x_rows;         // rows of y (= top_k * x_rows) and of x
+  int rows, x_rows;         // rows of y without the extra ones, and of x (with all that follow)
   const int32_t* offsets;   // nullable [E + 1]
   const int32_t* order;     // nullable [rows]
   int top_k;

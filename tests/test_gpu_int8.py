@@ -13,6 +13,9 @@ about |x| 2^-24 relative, |x| <= 88 where it matters: 2^-17).
 
 from __future__ import annotations
 
+import ctypes
+from pathlib import Path
+
 import numpy as np
 import pytest
 import torch
@@ -379,6 +382,105 @@ def test_grouped_weights_past_32_bits(dev):
         at = torch.arange(R, device=dev)
         ref, err = grouped_ref(x, w[-1:], [R], (at, at), None, None, xs, ws[-1:])
         within(y, ref, err)
+
+
+# ----------------------------------------------------------------------------- every form
+
+FORMS_HELPER = Path(__file__).resolve().parent / "gpu_helpers" / "libmatmulforms.so"
+FORMS = ["split", "whole", "wide", "128x64", "128x64 once", "256x128", "256x128 once", "256x256"]
+
+
+class FormArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "xs", "w", "ws", "offsets", "order", "row_weight", "extra_w",
+                                                "extra_ws", "y")]
+                + [(n, ctypes.c_int) for n in ("int8", "E", "N", "K", "rows", "x_rows", "top_k", "act", "extra",
+                                               "extra_x", "quantise", "out_f32")]
+                + [("limit", ctypes.c_float), ("extra_limit", ctypes.c_float)])
+
+
+def run_form(form, **args):
+    if not FORMS_HELPER.exists():
+        from tests.gpu_helpers import build_helpers  # built by __graft_entry__.build(); rebuilt if absent
+
+        build_helpers.build()
+    fn = ctypes.CDLL(str(FORMS_HELPER)).ftmoe_test_matmul_form
+    fn.argtypes = [ctypes.POINTER(FormArgs), ctypes.c_int, ctypes.c_void_p]
+    ptr = {k: v.data_ptr() if isinstance(v, torch.Tensor) else v for k, v in args.items()}
+    assert fn(ctypes.byref(FormArgs(**ptr)), FORMS.index(form), torch.cuda.current_stream().cuda_stream) == 0
+
+
+@pytest.mark.parametrize("gate", [False, True], ids=["plain", "gated"])
+@pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("form", FORMS)
+def test_forms(dev, form, int8, gate):
+    """Every form at the same ragged problem, whatever the rule would take: empty groups, blocks of one row to several,
+    rows in a routed order with several routes per token, one more group with a matrix and rows of its own behind."""
+    counts, k = [1, 0, 33, 5, 0, 270, 64, 129, 16], 2
+    E, R, extra = len(counts), sum(counts), 37
+    x_rows = R // k
+    for N, K in [(530, 1168), (40, 16), (1030, 384)]:
+        g = gen(dev, N)
+        if int8:
+            x, w = int8_rows(dev, g, x_rows + extra, K), int8_rows(dev, g, E + 1, N, K)
+            xs, ws = scales(dev, g, x_rows + extra), scales(dev, g, E + 1, N)
+        else:
+            x = torch.randn((x_rows + extra, K), generator=g, device=dev).to(torch.bfloat16)
+            w = torch.randn((E + 1, N, K), generator=g, device=dev).to(torch.bfloat16)
+            xs = ws = None
+        more = w[E].clone(), None if ws is None else ws[E].clone()
+        weight = None if gate else torch.rand((R,), generator=g, device=dev)
+        order = torch.randperm(R, generator=g, device=dev).to(torch.int32)
+        offsets = torch.tensor([0] + list(np.cumsum(counts)), dtype=torch.int32, device=dev)
+        n_out = N // 2 if gate else N
+        guard = torch.full((R + extra + 1, n_out), 7.0, dtype=torch.bfloat16, device=dev)
+        run_form(form, x=x, xs=xs, w=w, ws=ws, offsets=offsets, order=order, row_weight=weight, extra_w=more[0],
+                 extra_ws=more[1], y=guard, int8=int(int8), E=E, N=N, K=K, rows=R, x_rows=x_rows + extra, top_k=k,
+                 act=0 if gate else -1, extra=extra, extra_x=x_rows, quantise=0, out_f32=0, limit=0.0, extra_limit=0.0)
+        at = order.long()
+        act = "silu" if gate else None
+        ref, err = grouped_ref(x, w, counts, (at, at // k), act, weight, xs, ws)
+        within(guard[:R], ref, err)
+        at = torch.arange(extra, device=dev)
+        ref, err = grouped_ref(x[x_rows:], w[E:], [extra], (at, at), act, None, None if xs is None else xs[x_rows:],
+                               None if ws is None else ws[E:])
+        within(guard[R : R + extra], ref, err)
+        assert bool((guard[-1] == 7.0).all())
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_forms_dense_f32(dev, form):
+    """One group without offsets and order, float32 results."""
+    M, N, K = 301, 517, 1808
+    g = gen(dev, 11)
+    x, w, xs, ws = int8_rows(dev, g, M, K), int8_rows(dev, g, N, K), scales(dev, g, M), scales(dev, g, N)
+    y = torch.full((M + 1, N), 7.0, device=dev)
+    run_form(form, x=x, xs=xs, w=w, ws=ws, offsets=None, order=None, row_weight=None, extra_w=None, extra_ws=None, y=y,
+             int8=1, E=1, N=N, K=K, rows=M, x_rows=M, top_k=1, act=-1, extra=0, extra_x=0, quantise=0, out_f32=1,
+             limit=0.0, extra_limit=0.0)
+    ref = (x.double() @ w.double().T) * xs.double()[:, None] * ws.double()
+    within(y[:M], ref, ref.abs() * F32)
+    assert bool((y[M] == 7.0).all())
+
+
+@pytest.mark.parametrize("K", [16, 768, 2032, 2048])
+@pytest.mark.parametrize("form", ["split", "whole"])
+def test_forms_that_quantise(dev, form, K):
+    """bf16 rows quantised inside the product: the codes and scales of act_quant_int8, so the very results."""
+    counts = [3, 0, 1, 20]
+    E, R, N = len(counts), sum(counts), 200
+    g = gen(dev, K)
+    x = torch.randn((R, K), generator=g, device=dev).to(torch.bfloat16)
+    x[1] = 0
+    w, ws = int8_rows(dev, g, E, N, K), scales(dev, g, E, N)
+    offsets = torch.tensor([0] + list(np.cumsum(counts)), dtype=torch.int32, device=dev)
+    q, s = ops.act_quant_int8(x)
+    y = torch.full((2, R + 1, N), 7.0, dtype=torch.bfloat16, device=dev)
+    y[:, :R] = float("nan")
+    for i, (rows, xs) in enumerate([(x, None), (q, s)]):
+        run_form(form, x=rows, xs=xs, w=w, ws=ws, offsets=offsets, order=None, row_weight=None, extra_w=None,
+                 extra_ws=None, y=y[i], int8=1, E=E, N=N, K=K, rows=R, x_rows=R, top_k=1, act=-1, extra=0, extra_x=0,
+                 quantise=1 - i, out_f32=0, limit=0.0, extra_limit=0.0)
+    assert torch.equal(y[0], y[1]) and bool((y[:, R] == 7.0).all())
 
 
 # ----------------------------------------------------------------------------- the layer
