@@ -353,6 +353,24 @@ def test_grouped_offsets_are_cut(dev):
     assert bool((out[7:9] == 7.0).all())
 
 
+@pytest.mark.parametrize("R", [3, 40, 700])
+def test_grouped_views(dev, R):
+    """Scales, weights, order and offsets that begin 4 bytes into their memory, matrices that begin 16 into theirs."""
+    g = gen(dev, R)
+    E, N, K, off = 3, 72, 208, 1
+    x, w = int8_rows(dev, g, R + off, K)[off:], int8_rows(dev, g, E + off, N, K)[off:]
+    xs, ws = scales(dev, g, R + off)[off:], scales(dev, g, E * N + off)[off:].view(E, N)
+    weight = torch.rand((R + off,), generator=g, device=dev)[off:]
+    order = torch.randperm(R, generator=g, device=dev).to(torch.int32)
+    order = torch.cat([order[:1], order])[off:]
+    counts = [R // 3, 0, R - R // 3]
+    offsets = torch.tensor([0, 0] + list(np.cumsum(counts)), dtype=torch.int32, device=dev)[off:]
+    y = ops.grouped_matmul(x, w, offsets, order=order, x_scale=xs, w_scale=ws, row_weight=weight)
+    at = order.long()
+    ref, err = grouped_ref(x, w, counts, (at, at), None, weight, xs, ws)
+    within(y, ref, err)
+
+
 def test_grouped_nan_stays_in_its_row(dev):
     """A token's infinity or NaN reaches its own rows only; zeros beside NaN weights of other experts do not."""
     g = gen(dev, 4)
