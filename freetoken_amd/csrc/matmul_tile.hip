@@ -255,6 +255,7 @@ __global__ void __launch_bounds__(kWave* WR* WC) matmul_tile_kernel(MatmulArgs a
       const int col = 32 * CT * wc + 32 * i + r32;
       const float xs = INT8 ? s_xs(b)[col] : 1.0f;
       const float rw = a.row_weight ? s_rw(b)[col] : 1.0f;
+      const float by = GATE ? xs : xs * rw;
       const int r = a.out_f32 ? route_of(t, b, col) : 0;
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
@@ -266,14 +267,14 @@ __global__ void __launch_bounds__(kWave* WR* WC) matmul_tile_kernel(MatmulArgs a
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             float y = static_cast<float>(acc[j][i][4 * q + v]);
-            if (INT8) y *= wg[v] * xs;
+            if (INT8) y *= wg[v] * by;
             if constexpr (GATE) {
               float u = static_cast<float>(acc[RT / 2 + j][i][4 * q + v]);
               if (INT8) u *= wu[v] * xs;
               swiglu_clamp(limit, y, u);
               y = act_apply(a.act, y) * u;
             }
-            o[v] = y * rw;
+            o[v] = INT8 && !GATE ? y : y * rw;
           }
           if (!a.out_f32) {
             const int chunk = (4 * j + q) ^ (r32 & (NC - 1));
@@ -302,7 +303,9 @@ __global__ void __launch_bounds__(kWave* WR* WC) matmul_tile_kernel(MatmulArgs a
         const int n = nw + 8 * chunk;
         if (row < 0 || n >= n_out) continue;
         uint16_t* const dst = static_cast<uint16_t*>(a.y) + static_cast<size_t>(row) * n_out + n;
-        if (whole) {
+        if (whole && !GATE) {  // written once, past the caches (65536 rows, N 2048, K 768: 190, cached 211)
+          __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(dst));
+        } else if (whole) {    // (the activations are read again at once)
           *reinterpret_cast<u32x4*>(dst) = v;
         } else {
 #pragma unroll
