@@ -8,6 +8,9 @@
 // atomics, and the stable order.  Up to 2048 routes one workgroup does all of it in
 // one launch; beyond, workgroups of 2048 routes count first, and in a second launch
 // each adds up the counts before its own and places its routes.
+//
+// Bound by latency: 32 routes 3.5 us, 512 (with 64 tokens of 7168 quantised) 4.7 us,
+// 32768 4.9 + 6.4 us, 65536 (with 8192 tokens of 2048, 50 MB) 12.6 + 8.7 us.
 #include <algorithm>
 
 #include "quant_int8.h"
