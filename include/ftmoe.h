@@ -51,10 +51,16 @@ enum ftmoe_format {
   FTMOE_FMT_BF16 = 0,     /* bf16 weights */
   FTMOE_FMT_FP8_B128 = 1, /* e4m3 weights + float32 128x128 block scales */
   FTMOE_FMT_MXFP4 = 2,    /* e2m1 weights + e8m0 scale per 32 K (row-major "ds_fp4" layout) */
-  FTMOE_FMT_INT8 = 3      /* int8 weights + float32 scale per output channel (ftmoe_experts_int8, ftmoe_grouped_matmul) */
+  FTMOE_FMT_INT8 = 3      /* int8 weights + float32 scale per output channel (ftmoe_experts_int8,
+                             ftmoe_grouped_matmul) */
 };
 
-enum ftmoe_activation { FTMOE_ACT_NONE = -1 /* matrix products only */, FTMOE_ACT_SILU = 0, FTMOE_ACT_GELU = 1, FTMOE_ACT_GELU_TANH = 2 };
+enum ftmoe_activation {
+  FTMOE_ACT_NONE = -1, /* matrix products only */
+  FTMOE_ACT_SILU = 0,
+  FTMOE_ACT_GELU = 1,
+  FTMOE_ACT_GELU_TANH = 2
+};
 
 /* Indices of the int64 counters accumulated by ftmoe_slot_map (moe/offload_cache.py:205-229). */
 enum ftmoe_stat { FTMOE_STAT_ACTIVE = 0, FTMOE_STAT_MISS = 1, FTMOE_STAT_CALLS = 2, FTMOE_STAT_MISSED_ROUTES = 3 };
@@ -364,7 +370,8 @@ int ftmoe_group_routes(const int32_t* topk_ids, int numel, int num_experts, int3
 
 /* Matrix products grouped by expert, each with a ragged set of rows:
  *   y[r] = row_weight[r] * (x[r / top_k] . w[e]^T)   for r = order[i] and offsets[e] <= i < offsets[e + 1],
- * with the sums in float32 (bf16) or exact in 32-bit integers and scaled (int8). */
+ * with the sums in float32 (bf16) or exact in 32-bit integers and scaled (int8).
+ * num_experts <= 1023; x, and with an activation each matrix, below 2 GiB. */
 typedef struct ftmoe_grouped {
   int format;               /* FTMOE_FMT_BF16 or FTMOE_FMT_INT8: x and w */
   int num_experts, N, K;
@@ -387,7 +394,10 @@ int ftmoe_grouped_matmul(const ftmoe_grouped* args, ftmoe_stream_t stream);
  * and up rows, act(gate) * up is rounded to bf16 and quantised per route,
  * multiplied with the down rows and the router weight to a bf16 row, and a token's
  * rows (the last one the shared expert's: nullable, an INT8 bank of one row) are
- * summed in float32.  Ids outside [0, num_rows) are skipped.  num_rows <= 1023. */
+ * summed in float32.  Ids outside [0, num_rows) are skipped.  num_rows <= 1023;
+ * hidden and inter multiples of 16, at most 131056; x as int8, the activations
+ * of all routes (M top_k, and M for the shared expert) as int8 and each matrix
+ * below 2 GiB. */
 size_t ftmoe_experts_int8_workspace(int M, int top_k, const ftmoe_bank* bank, const ftmoe_bank* shared);
 int ftmoe_experts_int8(const void* x, int M, int top_k, const float* topk_w, const int32_t* topk_ids,
                        const ftmoe_bank* bank, const ftmoe_bank* shared, int activation, void* y, void* workspace,
@@ -467,7 +477,7 @@ int ftmoe_cpu_experts_submit(ftmoe_cpu_executor* ex, const ftmoe_bank* host_bank
 int ftmoe_cpu_experts_wait(ftmoe_cpu_executor* ex, void* job, ftmoe_stream_t stream);
 
 /* Instrumentation (no counterpart in the reference, whose NVTX ranges play this
- * role): between begin and end, every ftmoe_experts_* call made outside graph
+ * role): between begin and end, every decode and prefill expert call made outside graph
  * capture records a HIP event on its stream before its first kernel and after
  * each kernel.  end synchronises on those events, writes the summed
  * milliseconds of each stage (decode: align, gate_up, down, combine; prefill:
