@@ -295,22 +295,29 @@ def act_quant_fp8(x: torch.Tensor, mode: int = 0):
 # --------------------------------------------------------------------------- 8-bit integers, ragged groups
 
 
-def _one_device(first: torch.Tensor, *others: torch.Tensor | None) -> torch.device:
-    """The device that holds all the tensors."""
-    dev = first.device
-    for t in others:
-        if t is not None and t.device != dev:
+def _one_gpu(*tensors: torch.Tensor | None) -> torch.device:
+    """The device that holds all the tensors (the first is one)."""
+    dev = tensors[0].device
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda or not t.is_contiguous():
+            _require_gpu(t)
+        if t.device != dev:
             raise ValueError(f"tensors on different devices: {dev} and {t.device}")
     return dev
 
 
 def _launch(what: str, fn, dev: torch.device, *args) -> None:
-    """Calls the entry point with ``dev`` current and its current stream last."""
-    if torch._C._cuda_getDevice() == dev.index:  # (the guard object costs 1.4 us a call)
-        check(fn(*args, _stream(dev)), what)
+    """Calls the entry point with ``dev``, a tensor's device, current and its current stream last."""
+    index = dev.index
+    if torch._C._cuda_getDevice() == index:  # (the guard object costs 1.4 us a call)
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
-            check(fn(*args, _stream(dev)), what)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, what)
 
 
 def _act_code(activation: str | None) -> int:
@@ -330,10 +337,11 @@ def act_quant_int8(x: torch.Tensor):
         raise ValueError("x must be bfloat16")
     if x.dim() < 1:
         raise ValueError("x must have rows")
-    _require_gpu(x)
-    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    s = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    _launch("act_quant_int8", lib().ftmoe_act_quant_int8, x.device, _ptr(x), s.numel(), x.shape[-1], _ptr(q), _ptr(s))
+    dev = _one_gpu(x)
+    *lead, k = x.shape
+    q = torch.empty_like(x, dtype=torch.int8)  # (1 us less than torch.empty of the shape)
+    s = torch.empty(lead, dtype=torch.float32, device=dev)
+    _launch("act_quant_int8", lib().ftmoe_act_quant_int8, dev, x.data_ptr(), s.numel(), k, q.data_ptr(), s.data_ptr())
     return q, s
 
 
@@ -345,24 +353,26 @@ def matmul_int8(q: torch.Tensor, q_scale: torch.Tensor, w: torch.Tensor, w_scale
     and ``w_scale`` float32 [N]; K a multiple of 16.  With an ``activation`` the
     first N/2 rows of ``w`` are gate and the others up rows, and the result [M,
     N/2] is ``act(gate) * up``.  ``out_dtype`` (or ``out``'s) is bfloat16 or float32."""
-    if q.dtype != torch.int8 or w.dtype != torch.int8 or q.dim() != 2 or w.dim() != 2 or q.shape[1] != w.shape[1]:
+    if q.dtype != torch.int8 or w.dtype != torch.int8 or q.dim() != 2 or w.dim() != 2:
+        raise ValueError("q and w must be int8 [M, K] and [N, K]")
+    (m, k), (n, wk) = q.shape, w.shape
+    if k != wk:
         raise ValueError("q and w must be int8 [M, K] and [N, K]")
     if q_scale.dtype != torch.float32 or w_scale.dtype != torch.float32:
         raise ValueError("scales must be float32")
-    if q_scale.shape != q.shape[:1] or w_scale.shape != w.shape[:1]:
+    if q_scale.shape != (m,) or w_scale.shape != (n,):
         raise ValueError("one scale per row of q and of w")
     act = _act_code(activation)
-    _require_gpu(q, q_scale, w, w_scale, out)
-    (m, k), n = q.shape, w.shape[0]
-    dev = _one_device(q, q_scale, w, w_scale, out)
+    dev = _one_gpu(q, q_scale, w, w_scale, out)
     shape = (m, n if activation is None else n // 2)
     y = out if out is not None else torch.empty(shape, dtype=out_dtype, device=dev)
-    if y.dtype not in (torch.bfloat16, torch.float32):
+    dtype = y.dtype
+    if dtype != torch.bfloat16 and dtype != torch.float32:
         raise ValueError("the result is bfloat16 or float32")
-    if tuple(y.shape) != shape:
+    if out is not None and out.shape != shape:
         raise ValueError(f"out must be {shape}")
-    _launch("matmul_int8", lib().ftmoe_matmul_int8, dev, _ptr(q), _ptr(q_scale), _ptr(w), _ptr(w_scale), m, n, k, act,
-            _lib.DTYPE_F32 if y.dtype == torch.float32 else _lib.DTYPE_BF16, _ptr(y))
+    _launch("matmul_int8", lib().ftmoe_matmul_int8, dev, q.data_ptr(), q_scale.data_ptr(), w.data_ptr(),
+            w_scale.data_ptr(), m, n, k, act, _lib.DTYPE_F32 if dtype == torch.float32 else _lib.DTYPE_BF16, y.data_ptr())
     return y
 
 
@@ -374,8 +384,7 @@ def group_routes(topk_ids: torch.Tensor, num_experts: int):
     among those positions."""
     if topk_ids.dtype != torch.int32:
         raise ValueError("topk_ids must be int32")
-    _require_gpu(topk_ids)
-    dev, numel = topk_ids.device, topk_ids.numel()
+    dev, numel = _one_gpu(topk_ids), topk_ids.numel()
     order = torch.empty((numel,), dtype=torch.int32, device=dev)
     offsets = torch.empty((max(num_experts, 0) + 2,), dtype=torch.int32, device=dev)
     ws = torch.empty((lib().ftmoe_group_routes_workspace(numel, num_experts),), dtype=torch.uint8, device=dev)
@@ -419,9 +428,7 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, orde
     if row_weight is not None and (row_weight.dtype != torch.float32 or row_weight.numel() != rows):
         raise ValueError("row_weight must be float32 with one entry per row of the result")
     act = _act_code(activation)
-    tensors = (x, w, offsets, order, x_scale, w_scale, row_weight, out)
-    _require_gpu(*tensors)
-    dev = _one_device(*tensors)
+    dev = _one_gpu(x, w, offsets, order, x_scale, w_scale, row_weight, out)
     shape = (rows, n if activation is None else n // 2)
     if out is not None and (out.dtype != torch.bfloat16 or tuple(out.shape) != shape):
         raise ValueError(f"out must be bfloat16 {shape}")
@@ -746,7 +753,8 @@ def experts_int8(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.Tensor, 
         raise ValueError(f"Unsupported activation: {activation}")
     if bank.fmt != "int8" or (shared is not None and shared.fmt != "int8"):
         raise ValueError("experts_int8 takes int8 banks")
-    _require_gpu(x, topk_w, topk_ids, out)
+    dev = _one_gpu(x, topk_w, topk_ids, out, bank.gate_up, bank.down, bank.gate_up_scale, bank.down_scale,
+                   *((shared.gate_up, shared.down, shared.gate_up_scale, shared.down_scale) if shared else ()))
     m, k = topk_ids.shape
     if x.dim() != 2 or x.shape[0] != m:
         raise ValueError("Number of tokens mismatch")
@@ -758,8 +766,6 @@ def experts_int8(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.Tensor, 
     sb = shared.cstruct() if shared is not None else None
     bp = ctypes.byref(b)
     sp = ctypes.byref(sb) if sb is not None else None
-    dev = _one_device(x, topk_w, topk_ids, out, bank.gate_up, bank.down, bank.gate_up_scale, bank.down_scale,
-                      *((shared.gate_up, shared.down, shared.gate_up_scale, shared.down_scale) if shared else ()))
     # a workspace of the call's own: of the stream's pool, or of the graph's under capture
     ws = torch.empty((lib().ftmoe_experts_int8_workspace(m, k, bp, sp),), dtype=torch.uint8, device=dev)
     y = out if out is not None else torch.empty_like(x)
