@@ -1086,10 +1086,18 @@ int ftmoe_experts_int8(const void* x, int M, int top_k, const float* topk_w, con
   g.K = H;
   g.q = L.xq;
   g.scales = L.xs;
-  if (!run(ftmoe::launch_group_routes(g, L.hist, stream), "experts_int8 grouping and x quant")) return rc;
+  const bool down_quantises = ftmoe::launch_matmul_quantises(down);
+  if (down_quantises && ftmoe::launch_matmul_quantises(up) && (joined || !shared)) {  // (32 routes at most)
+    up.ids = down.ids = topk_ids;
+    up.quantise = 1;
+    up.x = static_cast<const uint8_t*>(x);
+    up.xs = nullptr;
+  } else if (!run(ftmoe::launch_group_routes(g, L.hist, stream), "experts_int8 grouping and x quant")) {
+    return rc;
+  }
   if (!run(ftmoe::launch_matmul(up, stream), "experts_int8 gate_up")) return rc;
   // (rows of skipped routes hold what the workspace held: quantised, never multiplied)
-  if (ftmoe::launch_matmul_quantises(down)) {
+  if (down_quantises) {
     down.quantise = 1;
     down.x = reinterpret_cast<const uint8_t*>(L.act);
     down.xs = nullptr;

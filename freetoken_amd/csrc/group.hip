@@ -13,6 +13,7 @@
 // 32768 4.9 + 6.4 us, 65536 (with 8192 tokens of 2048, 50 MB) 12.6 + 8.7 us.
 #include <algorithm>
 
+#include "matmul.h"
 #include "quant_int8.h"
 
 namespace ftmoe {
@@ -29,16 +30,6 @@ struct GroupShared {
   int scan[kGroupWaves];
   int sum[kCountMaxRows + 1], before[kCountMaxRows + 1];  // of every id: all routes, those of earlier workgroups
 };
-
-// Lanes of the wave whose id equals this lane's (ids below 2^bits), among those with valid set.
-__device__ __forceinline__ unsigned long long same_id(int id, bool valid, int bits) {
-  unsigned long long m = __ballot(valid);
-  for (int b = 0; b < bits; ++b) {
-    const unsigned long long set = __ballot((id >> b) & 1);
-    m &= (id >> b) & 1 ? set : ~set;
-  }
-  return m;
-}
 
 // Exclusive prefix of v over the workgroup's threads; the sum in *total.
 __device__ __forceinline__ int group_scan(int v, GroupShared& s, int* total) {

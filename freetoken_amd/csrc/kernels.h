@@ -287,6 +287,7 @@ struct MatmulArgs {
   int rows, x_rows;         // rows of y without the extra ones, and of x (with all that follow)
   const int32_t* offsets;   // nullable [E + 1]
   const int32_t* order;     // nullable [rows]
+  const int32_t* ids;       // with quantise, nullable [rows <= 64]: the group of every row, in the place of the two above
   int top_k;
   const float* row_weight;  // nullable [rows]
   int act;                  // -1: none, else Act
@@ -302,7 +303,7 @@ struct MatmulArgs {
   void* y;                  // [rows + extra, N] (N/2 with act)
 };
 hipError_t launch_matmul(const MatmulArgs& a, hipStream_t stream);
-// Whether the product (int8, without act) takes bf16 rows of x as they are.
+// Whether the product (int8) takes bf16 rows of x as they are.
 bool launch_matmul_quantises(const MatmulArgs& a);
 hipError_t launch_act_quant_int8(const uint16_t* x, int rows, int K, int8_t* q, float* scales, hipStream_t stream);
 // Routes by expert (group.hip), and beside it the quantisation of the tokens where x is given.

@@ -62,6 +62,16 @@ __device__ __forceinline__ void group_range(const MatmulArgs& a, int e, int& beg
   }
 }
 
+// Lanes of the wave whose id equals this lane's (ids below 2^bits), among those with valid set.
+__device__ __forceinline__ unsigned long long same_id(int id, bool valid, int bits) {
+  unsigned long long m = __ballot(valid);
+  for (int b = 0; b < bits; ++b) {
+    const unsigned long long set = __ballot((id >> b) & 1);
+    m &= (id >> b) & 1 ? set : ~set;
+  }
+  return m;
+}
+
 __host__ __device__ inline int group_count(const MatmulArgs& a) { return a.E + (a.extra > 0 ? 1 : 0); }
 
 // The streaming form, for few rows per group (matmul_stream.hip): a workgroup has

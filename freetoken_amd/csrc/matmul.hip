@@ -98,10 +98,10 @@ Form form_of(const MatmulArgs& a) {
 
 bool launch_matmul_quantises(const MatmulArgs& a) {
   const Form form = form_of(a);
-  // Saves a launch, but every workgroup quantises its group's rows anew.  An expert layer (us, with / without):
-  // 8 routes over 16 experts (H 1024, I 512) 16.6 / 17.9; over 128 (H 2048, I 768) 8 routes 21.1 / 22.8, 64 routes
-  // 60.7 / 55.2, 512 121 / 106.
-  return a.int8 && a.act < 0 && a.K <= kStreamQuantMaxK && a.rows <= 32 &&
+  // Saves a launch each, but every workgroup quantises its group's rows anew.  An expert layer (us, neither product /
+  // the down product / both): 8 routes over 16 experts (H 1024, I 512) 17.9 / 17.2 / 14.6; over 128 (H 2048, I 768)
+  // 8 routes 22.8 / 21.2 / 18.1, 32 routes - / 39.7 / 36.8, 64 routes 55.2 / 60.7, 512 routes 106 / 121.
+  return a.int8 && a.K <= kStreamQuantMaxK && a.rows <= 32 &&
          (form == Form::kSplit || form == Form::kWhole);
 }
 

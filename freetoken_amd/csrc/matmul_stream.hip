@@ -13,7 +13,9 @@
 //
 // QX: x is bf16.  The workgroup quantises its rows (quant_int8.h, the codes that
 // act_quant_int8 gives) into LDS while its first weights are on their way, which saves
-// a step of one or a few tokens the launch between an expert's two products.
+// a step of one or a few tokens the launch between an expert's two products, and
+// with the rows' experts found from their ids in every workgroup (ten ballots) also the
+// launch before the first.
 #include <algorithm>
 
 #include "kernels.h"
@@ -63,6 +65,40 @@ __device__ __forceinline__ bool find_block(const MatmulArgs& a, int block, int b
   return false;
 }
 
+// The same from the rows' ids (at most 64, one per lane): blocks of 16 rows, the groups
+// in the order of their first rows, and the row of this lane's column or -1.
+__device__ __forceinline__ bool find_rows(const MatmulArgs& a, int b, int& e, int& row) {
+  const int lane = lane_id(), r16 = lane & 15;
+  const int id = lane < a.rows ? a.ids[lane] : -1;
+  const bool valid = static_cast<uint32_t>(id) < static_cast<uint32_t>(a.E);
+  const unsigned long long same = same_id(id, valid, 32 - __builtin_clz(a.E));
+  const int rank = __popcll(same & ((1ull << lane) - 1));
+  const int nb = valid && rank == 0 ? (__popcll(same) + 15) / 16 : 0;
+  int sum = nb;
+#pragma unroll
+  for (int off = 1; off < kWave; off <<= 1) {
+    const int y = __shfl_up(sum, off, kWave);
+    if (lane >= off) sum += y;
+  }
+  const unsigned long long past = __ballot(sum > b);
+  if (!past) {
+    e = a.E;
+    const int i = a.rows + 16 * (b - __builtin_amdgcn_readlane(sum, kWave - 1)) + r16;
+    row = i < a.rows + a.extra ? i : -1;
+    return __ballot(row >= 0) != 0;
+  }
+  const int l = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<long long>(past)) - 1);
+  e = __builtin_amdgcn_readlane(id, l);
+  const int j = b - __builtin_amdgcn_readlane(sum - nb, l);
+  const bool mine = id == e && rank / 16 == j;
+  const int count = __popcll(__ballot(mine));
+  // lane numbers to the lanes of their columns, the others' to one that is not read
+  const int at = __builtin_amdgcn_ds_permute((mine ? rank % 16 : kWave - 1) * 4, lane);
+  const int r = __shfl(at, r16, kWave);
+  row = r16 < count ? r : -1;
+  return true;
+}
+
 template <bool INT8, bool GATE, bool QX, int RT, int CT, int S, int KS, int W>
 __global__ void __launch_bounds__(W* kWave) matmul_stream_kernel(MatmulArgs a) {
   using acc_t = typename Acc<INT8>::type;
@@ -70,15 +106,18 @@ __global__ void __launch_bounds__(W* kWave) matmul_stream_kernel(MatmulArgs a) {
   constexpr int kGroups = W / KS;  // waves that own rows of their own
   constexpr int kRed = KS > 1 ? W * RT * CT * kWave * 16 : 0;
   constexpr int kPerStep = 2 * RT + (QX ? 0 : 2 * CT);  // vector memory instructions of a step
-  // the quantised rows, their scales
-  constexpr int kXRow = kStreamQuantMaxK + 16, kXRows = QX ? 16 * CT * kXRow : 0;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[std::max(W * kRing, kRed) + kXRows + (QX ? 16 * CT * 4 : 0)];
-  uint8_t* const xq = lds + std::max(W * kRing, kRed);
-  float* const s_xs = reinterpret_cast<float*>(xq + kXRows);
+  // The quantised rows, chunk c (16 bytes) of row k at c ^ k % 16; their scales, where the rings were (two
+  // workgroups of gate and up rows just fit a CU).
+  constexpr int kXRow = kStreamQuantMaxK, kXRows = QX ? 16 * CT * kXRow : 0;
+  constexpr int kScales = QX ? 16 * CT * 4 : 0;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[std::max(W * kRing, kRed + kScales) + kXRows];
+  uint8_t* const xq = lds + std::max(W * kRing, kRed + kScales);
+  float* const s_xs = reinterpret_cast<float*>(lds + kRed);
   const int lane = lane_id(), r16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  int e, begin, end;
-  if (!find_block(a, 16 * CT, blockIdx.y, e, begin, end)) return;
+  int e, begin = 0, end = 0, listed = -1;
+  const bool by_id = QX && a.ids;
+  if (by_id ? !find_rows(a, blockIdx.y, e, listed) : !find_block(a, 16 * CT, blockIdx.y, e, begin, end)) return;
   const int n_out = GATE ? a.N / 2 : a.N;
   constexpr int NJ = GATE ? RT / 2 : RT;
   const int wk = wave % KS;
@@ -97,8 +136,8 @@ __global__ void __launch_bounds__(W* kWave) matmul_stream_kernel(MatmulArgs a) {
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
     const int i = begin + 16 * c + r16;
-    int r = -1;
-    if (i < end) {
+    int r = listed;
+    if (!by_id && i < end) {
       r = a.order && !extra ? a.order[i] : i;
       if (static_cast<uint32_t>(r) >= static_cast<uint32_t>(a.rows + a.extra)) r = -1;
     }
@@ -130,6 +169,7 @@ __global__ void __launch_bounds__(W* kWave) matmul_stream_kernel(MatmulArgs a) {
   constexpr int kMine = QX ? 16 * CT / W : 1, kPieces = QX ? kStreamQuantMaxK / 8 / kWave : 1;
   u32x4 raw[kMine][kPieces];
   int mine[kMine];
+  float scale[kMine];
   if constexpr (QX) {
 #pragma unroll
     for (int m = 0; m < kMine; ++m) {
@@ -166,11 +206,13 @@ __global__ void __launch_bounds__(W* kWave) matmul_stream_kernel(MatmulArgs a) {
     for (int c = 0; c < CT; ++c) acc[j][c] = acc_t{};
   auto compute = [&](int slot, int s) {
     if constexpr (QX) {  // (steps past the end, and past K in the last one, meet zero weights)
-      const uint8_t* const at = xq + r16 * kXRow + min(lo + s, nst - 1) * 128 + 16 * g;
+      const uint8_t* const at = xq + r16 * kXRow;
+      const int chunk = min(lo + s, nst - 1) * 8 + g;
 #pragma unroll
       for (int c = 0; c < CT; ++c)
 #pragma unroll
-        for (int p = 0; p < 2; ++p) xf[slot][c][p] = *reinterpret_cast<const u32x4*>(at + c * 16 * kXRow + 64 * p);
+        for (int p = 0; p < 2; ++p)
+          xf[slot][c][p] = *reinterpret_cast<const u32x4*>(at + c * 16 * kXRow + 16 * ((chunk + 4 * p) ^ r16));
     }
 #pragma unroll
     for (int j = 0; j < RT; ++j) {
@@ -191,6 +233,7 @@ __global__ void __launch_bounds__(W* kWave) matmul_stream_kernel(MatmulArgs a) {
   if constexpr (QX) {
 #pragma unroll
     for (int m = 0; m < kMine; ++m) {
+      scale[m] = 0.f;
       if (mine[m] < 0) continue;
       const int k = m * W + wave;
       uint32_t top = 0;
@@ -199,11 +242,12 @@ __global__ void __launch_bounds__(W* kWave) matmul_stream_kernel(MatmulArgs a) {
 #pragma unroll
         for (int w4 = 0; w4 < 4; ++w4) top = max_pair(top, raw[m][p][w4]);
       const RowCodes rc = row_codes(wave_max_pair(top));
-      if (lane == 0) s_xs[k] = rc.scale;
+      scale[m] = rc.scale;
 #pragma unroll
       for (int p = 0; p < kPieces; ++p)
         if (lane + p * kWave < a.K / 8)
-          *reinterpret_cast<uint2*>(xq + k * kXRow + 8 * (lane + p * kWave)) = rc.codes(raw[m][p]);
+          *reinterpret_cast<uint2*>(xq + k * kXRow + 16 * ((lane + p * kWave) / 2 ^ (k & 15)) + 8 * (lane & 1)) =
+              rc.codes(raw[m][p]);
     }
     wait_lgkm0();
     bare_barrier();
@@ -222,13 +266,18 @@ __global__ void __launch_bounds__(W* kWave) matmul_stream_kernel(MatmulArgs a) {
   // ---- the waves' sums through LDS; of the KS waves of the same rows, wave w finishes the tiles t with t % KS == w
   acc_t* const red = reinterpret_cast<acc_t*>(lds);
   const int w0 = wave - wk;
-  if constexpr (KS > 1) {
+  if constexpr (KS > 1 || QX) {
     wait_vm<0>();
     __syncthreads();
+    if constexpr (KS > 1)
 #pragma unroll
-    for (int j = 0; j < RT; ++j)
+      for (int j = 0; j < RT; ++j)
 #pragma unroll
-      for (int c = 0; c < CT; ++c) red[((wave * RT + j) * CT + c) * kWave + lane] = acc[j][c];
+        for (int c = 0; c < CT; ++c) red[((wave * RT + j) * CT + c) * kWave + lane] = acc[j][c];
+    if constexpr (QX)
+#pragma unroll
+      for (int m = 0; m < kMine; ++m)
+        if (lane == 0) s_xs[m * W + wave] = scale[m];
     __syncthreads();
   }
   auto sum = [&](int j, int c) {
@@ -250,19 +299,20 @@ __global__ void __launch_bounds__(W* kWave) matmul_stream_kernel(MatmulArgs a) {
       const acc_t su = GATE ? sum(NJ + j, c) : sg;
       const float xs = QX ? s_xs[16 * c + r16] : INT8 ? a.xs[x_row(r)] : 1.0f;
       const float wt = a.row_weight && r < a.rows ? a.row_weight[r] : 1.0f;
+      const float by = GATE ? xs : xs * wt;  // (the same products in every form)
       float o[4];
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         const int f = min(nn + v, n_out - 1);
         float y = static_cast<float>(sg[v]);
-        if (INT8) y *= ws[f] * xs;
+        if (INT8) y *= ws[f] * by;
         if constexpr (GATE) {
           float u = static_cast<float>(su[v]);
           if (INT8) u *= ws[n_out + f] * xs;
           swiglu_clamp(limit, y, u);
           y = act_apply(a.act, y) * u;
         }
-        o[v] = y * wt;
+        o[v] = INT8 && !GATE ? y : y * wt;
       }
       const size_t at = static_cast<size_t>(r) * n_out + nn;
       if (n_out % 4 == 0) {
@@ -306,9 +356,12 @@ hipError_t launch_stream(const MatmulArgs& a, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_matmul_stream(const MatmulArgs& a, StreamShape shape, hipStream_t stream) {
-  if (a.quantise)
+  if (a.quantise && a.act < 0)
     return shape == kStreamWhole ? launch_one<true, false, true, 1, 1, 3, 1, 4>(a, stream)
                                  : launch_one<true, false, true, 1, 1, 3, 4, 4>(a, stream);
+  if (a.quantise)
+    return shape == kStreamWhole ? launch_one<true, true, true, 2, 1, 3, 1, 4>(a, stream)
+                                 : launch_one<true, true, true, 2, 1, 3, 4, 4>(a, stream);
   switch (shape) {
     case kStreamSplit: return launch_stream<1, 1, 3, 4, 4>(a, stream);
     case kStreamWhole: return launch_stream<1, 1, 3, 1, 4>(a, stream);

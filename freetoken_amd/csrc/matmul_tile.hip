@@ -8,7 +8,8 @@
 // tile to tile (the workgroups are persistent, one walk over the tiles each).
 //
 // int8 sums stay int32 to the end (exact), bf16 ones float32; a result is the sum
-// times its channel's and its row's scale (and weight), rounded to bf16 once.
+// times its channel's and its row's scale (and weight), rounded to bf16 once; the
+// factors are multiplied in the order of the streaming form.
 //
 // Two waves per SIMD and 32 x 32 MFMAs: one wave with 16 x 16 ones issues 2930 int8
 // T/s at most, two 4000, one with 32 x 32 ones 4100 (8192 x 4096 x 7168: 227 us with 4

@@ -13,6 +13,7 @@ struct FormArgs {
   const float* ws;
   const int32_t* offsets;
   const int32_t* order;
+  const int32_t* ids;
   const float* row_weight;
   const void* extra_w;
   const float* extra_ws;
@@ -35,6 +36,7 @@ extern "C" int ftmoe_test_matmul_form(const FormArgs* f, int form, hipStream_t s
   a.x_rows = f->x_rows;
   a.offsets = f->offsets;
   a.order = f->order;
+  a.ids = f->ids;
   a.top_k = f->top_k;
   a.row_weight = f->row_weight;
   a.act = f->act;

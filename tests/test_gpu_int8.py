@@ -409,8 +409,8 @@ FORMS = ["split", "whole", "wide", "128x64", "128x64 once", "256x128", "256x128 
 
 
 class FormArgs(ctypes.Structure):
-    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "xs", "w", "ws", "offsets", "order", "row_weight", "extra_w",
-                                                "extra_ws", "y")]
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "xs", "w", "ws", "offsets", "order", "ids", "row_weight",
+                                                "extra_w", "extra_ws", "y")]
                 + [(n, ctypes.c_int) for n in ("int8", "E", "N", "K", "rows", "x_rows", "top_k", "act", "extra",
                                                "extra_x", "quantise", "out_f32")]
                 + [("limit", ctypes.c_float), ("extra_limit", ctypes.c_float)])
@@ -451,7 +451,7 @@ def test_forms(dev, form, int8, gate):
         offsets = torch.tensor([0] + list(np.cumsum(counts)), dtype=torch.int32, device=dev)
         n_out = N // 2 if gate else N
         guard = torch.full((R + extra + 1, n_out), 7.0, dtype=torch.bfloat16, device=dev)
-        run_form(form, x=x, xs=xs, w=w, ws=ws, offsets=offsets, order=order, row_weight=weight, extra_w=more[0],
+        run_form(form, x=x, xs=xs, w=w, ws=ws, offsets=offsets, order=order, ids=None, row_weight=weight, extra_w=more[0],
                  extra_ws=more[1], y=guard, int8=int(int8), E=E, N=N, K=K, rows=R, x_rows=x_rows + extra, top_k=k,
                  act=0 if gate else -1, extra=extra, extra_x=x_rows, quantise=0, out_f32=0, limit=0.0, extra_limit=0.0)
         at = order.long()
@@ -472,8 +472,8 @@ def test_forms_dense_f32(dev, form):
     g = gen(dev, 11)
     x, w, xs, ws = int8_rows(dev, g, M, K), int8_rows(dev, g, N, K), scales(dev, g, M), scales(dev, g, N)
     y = torch.full((M + 1, N), 7.0, device=dev)
-    run_form(form, x=x, xs=xs, w=w, ws=ws, offsets=None, order=None, row_weight=None, extra_w=None, extra_ws=None, y=y,
-             int8=1, E=1, N=N, K=K, rows=M, x_rows=M, top_k=1, act=-1, extra=0, extra_x=0, quantise=0, out_f32=1,
+    run_form(form, x=x, xs=xs, w=w, ws=ws, offsets=None, order=None, ids=None, row_weight=None, extra_w=None,
+             extra_ws=None, y=y, int8=1, E=1, N=N, K=K, rows=M, x_rows=M, top_k=1, act=-1, extra=0, extra_x=0, quantise=0, out_f32=1,
              limit=0.0, extra_limit=0.0)
     ref = (x.double() @ w.double().T) * xs.double()[:, None] * ws.double()
     within(y[:M], ref, ref.abs() * F32)
@@ -495,10 +495,38 @@ def test_forms_that_quantise(dev, form, K):
     y = torch.full((2, R + 1, N), 7.0, dtype=torch.bfloat16, device=dev)
     y[:, :R] = float("nan")
     for i, (rows, xs) in enumerate([(x, None), (q, s)]):
-        run_form(form, x=rows, xs=xs, w=w, ws=ws, offsets=offsets, order=None, row_weight=None, extra_w=None,
+        run_form(form, x=rows, xs=xs, w=w, ws=ws, offsets=offsets, order=None, ids=None, row_weight=None, extra_w=None,
                  extra_ws=None, y=y[i], int8=1, E=E, N=N, K=K, rows=R, x_rows=R, top_k=1, act=-1, extra=0, extra_x=0,
                  quantise=1 - i, out_f32=0, limit=0.0, extra_limit=0.0)
     assert torch.equal(y[0], y[1]) and bool((y[:, R] == 7.0).all())
+
+
+@pytest.mark.parametrize("rows,k,E,extra", [(1, 1, 1, 0), (8, 8, 128, 1), (32, 8, 3, 4), (64, 2, 16, 33), (64, 1, 1, 0),
+                                            (20, 4, 1023, 0), (6, 3, 5, 2)])
+@pytest.mark.parametrize("gate", [False, True], ids=["plain", "gated"])
+@pytest.mark.parametrize("form", ["split", "whole"])
+def test_forms_by_id(dev, form, gate, rows, k, E, extra):
+    """Groups found from the rows' ids (some of no group): the very results of listed groups on quantised rows."""
+    N, K, tokens = 74, 592, rows // k
+    g, rng = gen(dev, rows + E), np.random.default_rng(rows + E)
+    x = torch.randn((tokens + extra, K), generator=g, device=dev).to(torch.bfloat16)
+    w, ws = int8_rows(dev, g, E + 1, N, K), scales(dev, g, E + 1, N)
+    flat = rng.integers(0, E, size=rows).astype(np.int32)
+    flat[rng.random(rows) < 0.15] = -1
+    flat[rng.random(rows) < 0.1] = E
+    ids = torch.from_numpy(flat).to(dev)
+    weight = None if gate else torch.rand((rows,), generator=g, device=dev)
+    order, offsets = ops.group_routes(ids, E)
+    q, s = ops.act_quant_int8(x)
+    more = w[E].clone(), ws[E].clone()
+    y = torch.full((2, rows + extra + 1, N // 2 if gate else N), 7.0, dtype=torch.bfloat16, device=dev)
+    for i, rows_of in enumerate([dict(x=x, xs=None, offsets=None, order=None, ids=ids),
+                                 dict(x=q, xs=s, offsets=offsets, order=order, ids=None)]):
+        run_form(form, w=w, ws=ws, row_weight=weight, extra_w=more[0], extra_ws=more[1], y=y[i], int8=1, E=E, N=N, K=K,
+                 rows=rows, x_rows=tokens + extra, top_k=k, act=0 if gate else -1, extra=extra, extra_x=tokens,
+                 quantise=1 - i, out_f32=0, limit=0.0, extra_limit=0.0, **rows_of)
+    skipped = torch.from_numpy((flat < 0) | (flat >= E)).to(dev)
+    assert torch.equal(y[0], y[1]) and bool((y[0, :rows][skipped] == 7.0).all()) and bool((y[0, -1] == 7.0).all())
 
 
 # ----------------------------------------------------------------------------- the layer
@@ -688,3 +716,19 @@ def test_two_streams_at_once(dev):
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("shared", [False, True], ids=["routed", "shared"])
+@pytest.mark.parametrize("H,I,E,k", [(1024, 512, 16, 2), (2048, 768, 128, 8), (2064, 528, 12, 3)])
+def test_layer_does_not_depend_on_the_batch(dev, H, I, E, k, shared):
+    """Integer sums and one order of roundings in every form: a token's result is the same alone, in a step of a few
+    and in a batch of hundreds."""
+    g = gen(dev, H + E)
+    bank = make_bank(dev, g, E, H, I)
+    sb = make_bank(dev, g, 1, H, I) if shared else None
+    x = torch.randn((600, H), generator=g, device=dev).to(torch.bfloat16)
+    tw, ids = routing(dev, g, 600, k, E)
+    whole = ops.experts_int8(x, tw, ids, bank, shared=sb)
+    for first, n in [(0, 1), (1, 2), (7, 4), (30, 9), (64, 40), (300, 299)]:
+        part = slice(first, first + n)
+        assert torch.equal(ops.experts_int8(x[part], tw[part], ids[part], bank, shared=sb), whole[part]), n
