@@ -47,6 +47,9 @@ __device__ __forceinline__ typename Acc32<INT8>::type mma32(u32x4 a, u32x4 b, ty
                                                    0);
 }
 
+// silu by the reciprocal instruction (off by about 2^-23), as every form takes it.
+__device__ __forceinline__ float silu_of(float g) { return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g)); }
+
 // Rows [begin, end) of group e in the grouped order, cut to [0, rows] whatever
 // the offsets hold; group E is the extra one.
 __device__ __forceinline__ void group_range(const MatmulArgs& a, int e, int& begin, int& end) {

@@ -23,6 +23,7 @@
 // results, 4 us a tile, overlap with neither.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "kernels.h"
 #include "lds_ring.h"
@@ -254,7 +255,8 @@ __global__ void __launch_bounds__(kWave* WR* WC) matmul_tile_kernel(MatmulArgs a
   // 32i + r32 of its wave.  bf16 results are staged in LDS (stg, which no copy
   // targets before the next tile's K loop; every wave in its own part) and stored
   // as 16-byte pieces of contiguous rows.
-  auto epilogue = [&](const MTile& t, int b, uint8_t* stg) {
+  // silu: known to be the activation (chosen once a tile, not once a value: 65536 rows, N 1536, K 2048 303, else 315).
+  auto epilogue = [&](const MTile& t, int b, uint8_t* stg, auto silu) {
     constexpr int NJ = GATE ? RT / 2 : RT;
     constexpr int RB = 64 * NJ;          // bytes of a row of y that a wave holds
     constexpr int NC = 4 * NJ;           // 16-byte chunks of it
@@ -287,7 +289,7 @@ __global__ void __launch_bounds__(kWave* WR* WC) matmul_tile_kernel(MatmulArgs a
               float u = static_cast<float>(acc[RT / 2 + j][i][4 * q + v]);
               if (INT8) u *= wu[v] * xs;
               swiglu_clamp(limit, y, u);
-              y = act_apply(a.act, y) * u;
+              y = (silu.value ? silu_of(y) : act_apply(a.act, y)) * u;
             }
             o[v] = INT8 && !GATE ? y : y * rw;
           }
@@ -389,7 +391,9 @@ __global__ void __launch_bounds__(kWave* WR* WC) matmul_tile_kernel(MatmulArgs a
       wait_lgkm0();
       bare_barrier();
     }
-    epilogue(cur, buf, t_lds + ring<S>(g0 + nkb + D) * L::kStage);
+    uint8_t* const stg = t_lds + ring<S>(g0 + nkb + D) * L::kStage;
+    if (!GATE || a.act == ACT_SILU) epilogue(cur, buf, stg, std::true_type{});
+    else epilogue(cur, buf, stg, std::false_type{});
     if (!has_next) break;
     ahead = cross;
     cur = nxt;
