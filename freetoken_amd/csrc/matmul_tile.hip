@@ -255,8 +255,10 @@ __global__ void __launch_bounds__(kWave* WR* WC) matmul_tile_kernel(MatmulArgs a
   // 32i + r32 of its wave.  bf16 results are staged in LDS (stg, which no copy
   // targets before the next tile's K loop; every wave in its own part) and stored
   // as 16-byte pieces of contiguous rows.
-  // silu: known to be the activation (chosen once a tile, not once a value: 65536 rows, N 1536, K 2048 303, else 315).
-  auto epilogue = [&](const MTile& t, int b, uint8_t* stg, auto silu) {
+  // plain: the results are bf16, an activation silu without a limit (chosen once a tile, not once a value: 65536 rows,
+  // N 1536, K 2048 303, else 315).
+  auto epilogue = [&](const MTile& t, int b, uint8_t* stg, auto plain) {
+    const bool out_f32 = !plain.value && a.out_f32;
     constexpr int NJ = GATE ? RT / 2 : RT;
     constexpr int RB = 64 * NJ;          // bytes of a row of y that a wave holds
     constexpr int NC = 4 * NJ;           // 16-byte chunks of it
@@ -266,34 +268,43 @@ __global__ void __launch_bounds__(kWave* WR* WC) matmul_tile_kernel(MatmulArgs a
     static_assert(WR * WC * 32 * RB <= L::kStage, "the staging areas fit a stage");
     const bool whole = n_out % 8 == 0;
     const float limit = t.e == E ? a.extra_limit : a.limit;
-    const float* const wsp = s_ws(b) + 32 * RT * wr + 4 * half;
+    f32x4 ws[RT][4];  // read once for all columns
+    if (INT8) {
+      const float* const wsp = s_ws(b) + 32 * RT * wr + 4 * half;
+#pragma unroll
+      for (int j = 0; j < RT; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) ws[j][q] = *reinterpret_cast<const f32x4*>(wsp + 32 * j + 8 * q);
+    }
 #pragma unroll
     for (int i = 0; i < CT; ++i) {
       const int col = 32 * CT * wc + 32 * i + r32;
       const float xs = INT8 ? s_xs(b)[col] : 1.0f;
       const float rw = a.row_weight ? s_rw(b)[col] : 1.0f;
       const float by = GATE ? xs : xs * rw;
-      const int r = a.out_f32 ? route_of(t, b, col) : 0;
+      const int r = out_f32 ? route_of(t, b, col) : 0;
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           float o[4];
-          const f32x4 wg = INT8 ? *reinterpret_cast<const f32x4*>(wsp + 32 * j + 8 * q) : f32x4{1.f, 1.f, 1.f, 1.f};
-          const f32x4 wu = INT8 && GATE ? *reinterpret_cast<const f32x4*>(wsp + 32 * (RT / 2 + j) + 8 * q) : wg;
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             float y = static_cast<float>(acc[j][i][4 * q + v]);
-            if (INT8) y *= wg[v] * by;
+            if (INT8) y *= ws[j][q][v] * by;
             if constexpr (GATE) {
               float u = static_cast<float>(acc[RT / 2 + j][i][4 * q + v]);
-              if (INT8) u *= wu[v] * xs;
-              swiglu_clamp(limit, y, u);
-              y = (silu.value ? silu_of(y) : act_apply(a.act, y)) * u;
+              if (INT8) u *= ws[RT / 2 + j][q][v] * xs;
+              if constexpr (plain.value) {
+                y = silu_of(y) * u;
+              } else {
+                swiglu_clamp(limit, y, u);
+                y = (a.act == ACT_SILU ? silu_of(y) : act_apply(a.act, y)) * u;
+              }
             }
             o[v] = INT8 && !GATE ? y : y * rw;
           }
-          if (!a.out_f32) {
+          if (!out_f32) {
             const int chunk = (4 * j + q) ^ (r32 & (NC - 1));
             *reinterpret_cast<uint2*>(mine + r32 * RB + chunk * 16 + half * 8) =
                 uint2{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
@@ -309,7 +320,7 @@ __global__ void __launch_bounds__(kWave* WR* WC) matmul_tile_kernel(MatmulArgs a
             }
           }
         }
-      if (a.out_f32) continue;
+      if (out_f32) continue;
       __builtin_amdgcn_wave_barrier();
       __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
 #pragma unroll
@@ -392,7 +403,8 @@ __global__ void __launch_bounds__(kWave* WR* WC) matmul_tile_kernel(MatmulArgs a
       bare_barrier();
     }
     uint8_t* const stg = t_lds + ring<S>(g0 + nkb + D) * L::kStage;
-    if (!GATE || a.act == ACT_SILU) epilogue(cur, buf, stg, std::true_type{});
+    const float limit = cur.e == E ? a.extra_limit : a.limit;
+    if (!a.out_f32 && (!GATE || (a.act == ACT_SILU && !(limit > 0.f)))) epilogue(cur, buf, stg, std::true_type{});
     else epilogue(cur, buf, stg, std::false_type{});
     if (!has_next) break;
     ahead = cross;
