@@ -17,10 +17,10 @@
 // stages, 256 x 128 three; 128 x 64 leave room for a second workgroup on the CU, which
 // multiplies while the first one stores.
 //
-// What bounds it: 65536 rows over 128 experts, N 2048, K 768 (256 x 128) take 185 us; its
+// What bounds it: 65536 rows over 128 experts, N 2048, K 768 (256 x 128) take 168 us; its
 // MFMAs and LDS reads alone 93, its copies alone 103 (66 where every tile reads the
 // same lines: they wait for lines that miss L2, two steps ahead fill the LDS), and the
-// results, 4 us a tile, overlap with neither.
+// results overlap with neither.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
