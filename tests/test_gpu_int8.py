@@ -732,3 +732,40 @@ def test_layer_does_not_depend_on_the_batch(dev, H, I, E, k, shared):
     for first, n in [(0, 1), (1, 2), (7, 4), (30, 9), (64, 40), (300, 299)]:
         part = slice(first, first + n)
         assert torch.equal(ops.experts_int8(x[part], tw[part], ids[part], bank, shared=sb), whole[part]), n
+
+
+@pytest.mark.parametrize("M", [3, 4, 90])
+def test_layer_odd_tokens(dev, M):
+    """A token of no expert is zero, one with an infinity or a NaN is NaN in its own row alone; the result may be
+    written over the tokens; a step in which no token has an expert."""
+    g = gen(dev, M)
+    E, H, I, k = 24, 512, 384, 4
+    bank = make_bank(dev, g, E, H, I)
+    x = torch.randn((M, H), generator=g, device=dev).to(torch.bfloat16)
+    tw, ids = routing(dev, g, M, k, E)
+    fine = ops.experts_int8(x, tw, ids, bank)
+    assert bool(torch.isfinite(fine).all())
+    bad = x.clone()
+    bad[1, 5], bad[2, 0] = float("nan"), float("-inf")
+    ids[0] = -1
+    y = ops.experts_int8(bad, tw, ids, bank)
+    assert not y[0].any() and bool(torch.isnan(y[1:3]).all()) and torch.equal(y[3:], fine[3:])
+    ids[0] = E + 5
+    assert ops.experts_int8(x, tw, ids, bank, out=x) is x
+    assert not x[0].any() and torch.equal(x[1:], fine[1:])
+    assert not ops.experts_int8(x, tw, torch.full_like(ids, E), bank).any()
+
+
+def test_layer_with_a_limit_in_a_small_step(dev):
+    """Clamped SwiGLU, the shared expert's limit its own, the same in a small step as in a batch."""
+    g = gen(dev, 21)
+    E, H, I, k = 16, 1024, 512, 2
+    bank, shared = make_bank(dev, g, E, H, I), make_bank(dev, g, 1, H, I)
+    bank.swiglu_limit, shared.swiglu_limit = 0.75, 7.0
+    x = torch.randn((400, H), generator=g, device=dev).to(torch.bfloat16)
+    tw, ids = routing(dev, g, 400, k, E)
+    whole = ops.experts_int8(x, tw, ids, bank, shared=shared)
+    for part in (slice(0, 1), slice(1, 12), slice(100, 400)):
+        assert torch.equal(ops.experts_int8(x[part], tw[part], ids[part], bank, shared=shared), whole[part])
+    bank.swiglu_limit = shared.swiglu_limit = 0.0
+    assert not torch.equal(ops.experts_int8(x, tw, ids, bank, shared=shared), whole)
