@@ -129,6 +129,8 @@ SIGNATURES = {
     "ftmoe_grouped_matmul": (_i, [ctypes.POINTER(FtmoeGrouped), _vp]),
     "ftmoe_experts_int8_workspace": (_sz, [_i, _i, _bp, _bp]),
     "ftmoe_experts_int8": (_i, [_vp, _i, _i, _vp, _vp, _bp, _bp, _i, _vp, _vp, _sz, _vp]),
+    "ftmoe_experts_int8_rows_workspace": (_sz, [_i, _i, _bp, _bp, _i]),
+    "ftmoe_experts_int8_rows": (_i, [_vp, _i, _i, _vp, _vp, _bp, _bp, _i, _i, _vp, _vp, _sz, _vp]),
     "ftmoe_cpu_executor_create": (_vp, [_i]),
     "ftmoe_cpu_executor_destroy": (_i, [_vp, _i]),
     "ftmoe_cpu_executor_healthy": (_i, [_vp]),

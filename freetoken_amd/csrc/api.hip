@@ -855,11 +855,11 @@ struct Int8Layout {
   uint16_t* act;     // [routes, inter], then the shared expert's [M, its inter]
   int8_t* actq;
   float* as;         // [routes + M]
-  uint16_t* routes;  // [routes + M, hidden]
+  uint8_t* routes;   // [routes + M, hidden] of the rows' type
   size_t bytes;
 };
 
-Int8Layout int8_layout(void* ws, int M, int k, const ftmoe_bank* bank, const ftmoe_bank* shared) {
+Int8Layout int8_layout(void* ws, int M, int k, const ftmoe_bank* bank, const ftmoe_bank* shared, int route_dtype) {
   Int8Layout L{};
   Carver c{static_cast<uint8_t*>(ws)};
   const int numel = M * k;
@@ -873,7 +873,7 @@ Int8Layout int8_layout(void* ws, int M, int k, const ftmoe_bank* bank, const ftm
   L.act = c.take<uint16_t>(act);
   L.actq = c.take<int8_t>(act);
   L.as = c.take<float>(rows);
-  L.routes = c.take<uint16_t>(rows * H);
+  L.routes = c.take<uint8_t>(rows * H * (route_dtype == FTMOE_DTYPE_F32 ? 4 : 2));
   L.bytes = c.off;
   return L;
 }
@@ -973,14 +973,26 @@ int ftmoe_grouped_matmul(const ftmoe_grouped* g, ftmoe_stream_t stream) {
   return check_hip(ftmoe::launch_matmul(a, stream), "grouped_matmul launch");
 }
 
-size_t ftmoe_experts_int8_workspace(int M, int top_k, const ftmoe_bank* bank, const ftmoe_bank* shared) {
+size_t ftmoe_experts_int8_rows_workspace(int M, int top_k, const ftmoe_bank* bank, const ftmoe_bank* shared,
+                                         int route_dtype) {
   if (!bank || M <= 0 || top_k <= 0) return 0;
-  return int8_layout(nullptr, M, top_k, bank, shared).bytes;
+  return int8_layout(nullptr, M, top_k, bank, shared, route_dtype).bytes;
+}
+
+size_t ftmoe_experts_int8_workspace(int M, int top_k, const ftmoe_bank* bank, const ftmoe_bank* shared) {
+  return ftmoe_experts_int8_rows_workspace(M, top_k, bank, shared, FTMOE_DTYPE_BF16);
 }
 
 int ftmoe_experts_int8(const void* x, int M, int top_k, const float* topk_w, const int32_t* topk_ids,
                        const ftmoe_bank* bank, const ftmoe_bank* shared, int activation, void* y, void* workspace,
                        size_t workspace_bytes, ftmoe_stream_t stream) {
+  return ftmoe_experts_int8_rows(x, M, top_k, topk_w, topk_ids, bank, shared, activation, FTMOE_DTYPE_BF16, y, workspace,
+                                 workspace_bytes, stream);
+}
+
+int ftmoe_experts_int8_rows(const void* x, int M, int top_k, const float* topk_w, const int32_t* topk_ids,
+                            const ftmoe_bank* bank, const ftmoe_bank* shared, int activation, int route_dtype, void* y,
+                            void* workspace, size_t workspace_bytes, ftmoe_stream_t stream) {
   int rc = check_int8_bank(bank, "routed", false);
   if (rc) return rc;
   if (shared) {
@@ -993,16 +1005,19 @@ int ftmoe_experts_int8(const void* x, int M, int top_k, const float* topk_w, con
     return fail(FTMOE_ERR_INVALID, "experts_int8: M=%d top_k=%d", M, top_k);
   if (activation < FTMOE_ACT_SILU || activation > FTMOE_ACT_GELU_TANH)
     return fail(FTMOE_ERR_UNSUPPORTED, "experts_int8: activation %d", activation);
+  if (route_dtype != FTMOE_DTYPE_BF16 && route_dtype != FTMOE_DTYPE_F32)
+    return fail(FTMOE_ERR_UNSUPPORTED, "experts_int8: dtype %d of the routes' rows", route_dtype);
   rc = check_limit(bank, shared, activation, "experts_int8");
   if (rc) return rc;
   if (M == 0) return FTMOE_OK;
   if (!x || !topk_w || !topk_ids || !y) return fail(FTMOE_ERR_INVALID, "experts_int8: NULL pointer");
   if (!aligned16(x) || !aligned16(y)) return fail(FTMOE_ERR_UNSUPPORTED, "experts_int8: x and y must be 16-byte aligned");
-  const size_t need = int8_layout(nullptr, M, top_k, bank, shared).bytes;
+  const size_t need = int8_layout(nullptr, M, top_k, bank, shared, route_dtype).bytes;
   if (!workspace || workspace_bytes < need)
     return fail(FTMOE_ERR_WORKSPACE, "experts_int8: workspace %zu < %zu bytes", workspace_bytes, need);
-  const Int8Layout L = int8_layout(workspace, M, top_k, bank, shared);
+  const Int8Layout L = int8_layout(workspace, M, top_k, bank, shared, route_dtype);
   const int numel = M * top_k, H = bank->hidden;
+  const bool rows_f32 = route_dtype == FTMOE_DTYPE_F32;
 
   // the two products of one bank's rows
   ftmoe::MatmulArgs up{}, down{};
@@ -1032,6 +1047,7 @@ int ftmoe_experts_int8(const void* x, int M, int top_k, const float* topk_w, con
   down.top_k = 1;
   down.act = FTMOE_ACT_NONE;
   down.row_weight = topk_w;
+  down.out_f32 = rows_f32;
   down.y = L.routes;
   // The shared expert: one more group of both products where its matrices have the
   // routed shape, else products of its own.
@@ -1064,7 +1080,7 @@ int ftmoe_experts_int8(const void* x, int M, int top_k, const float* topk_w, con
     sh_down.ws = static_cast<const float*>(shared->down_scale);
     sh_down.K = shared->inter;
     sh_down.row_weight = nullptr;
-    sh_down.y = L.routes + static_cast<size_t>(numel) * H;
+    sh_down.y = L.routes + static_cast<size_t>(numel) * H * (rows_f32 ? 4 : 2);
   }
   for (const ftmoe::MatmulArgs* a : {&up, &down, &sh_up, &sh_down}) {
     rc = check_product(*a, "experts_int8");
@@ -1113,7 +1129,7 @@ int ftmoe_experts_int8(const void* x, int M, int top_k, const float* topk_w, con
       return rc;
     if (!run(ftmoe::launch_matmul(sh_down, stream), "experts_int8 shared down")) return rc;
   }
-  run(ftmoe::launch_combine_routes(L.routes, topk_ids, bank->num_rows, shared != nullptr, M, top_k, H,
+  run(ftmoe::launch_combine_routes(L.routes, rows_f32, topk_ids, bank->num_rows, shared != nullptr, M, top_k, H,
                                    static_cast<uint16_t*>(y), stream),
       "experts_int8 combine");
   return rc;

@@ -320,9 +320,9 @@ struct GroupArgs {
 size_t group_hist_ints(int numel, int num_experts);  // workspace of launch_group_routes
 hipError_t launch_group_routes(const GroupArgs& a, int32_t* hist, hipStream_t stream);
 
-// The routes' rows of every token (ids outside [0, num_rows) skipped) and with shared its row behind all of those,
-// M k + t, summed in float32 and rounded once.
-hipError_t launch_combine_routes(const uint16_t* routes, const int32_t* ids, int num_rows, bool shared, int M,
+// The routes' rows of every token, bf16 or float32 (ids outside [0, num_rows) skipped), and with shared its row behind
+// all of those, M k + t, summed in float32 and rounded once.
+hipError_t launch_combine_routes(const void* routes, bool f32, const int32_t* ids, int num_rows, bool shared, int M,
                                  int k, int H, uint16_t* y, hipStream_t stream);
 
 hipError_t launch_combine(const uint16_t* ic3, const int32_t* ids, int num_rows, const uint16_t* sh_out, int M,

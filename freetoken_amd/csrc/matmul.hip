@@ -18,11 +18,28 @@ namespace {
 
 constexpr int kCombineThreads = 64;  // (a decode step has few: spread over the CUs)
 
+// Eight values of a route's row, past the caches: it is read once.
+template <typename T>
+__device__ __forceinline__ void load_row8(const T* p, u32x4 (&v)[sizeof(T) / 2]) {
+#pragma unroll
+  for (size_t i = 0; i < sizeof(T) / 2; ++i) v[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p) + i);
+}
+
+template <typename T>
+__device__ __forceinline__ void add_row8(float (&acc)[8], const u32x4 (&v)[sizeof(T) / 2]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (sizeof(T) == 4) acc[i] += __uint_as_float(v[i / 4][i % 4]);
+    else acc[i] += __uint_as_float(i % 2 ? v[0][i / 2] & 0xffff0000u : v[0][i / 2] << 16);
+  }
+}
+
 // y[t] = bf16(sum of the routes' rows in route order, then the shared row M k + t),
-// routes with ids outside [0, num_rows) skipped; H a multiple of 8.  The rows of
-// eight routes are read before the first is added.  Bound by reading them: 8192 x 8
-// rows of 2048 49 us (6.1 TB/s, part of it from the memory-side cache).
-__global__ void __launch_bounds__(kCombineThreads) combine_routes_kernel(const uint16_t* __restrict__ routes,
+// routes with ids outside [0, num_rows) skipped; H a multiple of 8; rows of T, bf16 (uint16_t) or float32.
+// The rows of eight routes are read before the first is added.  Bound by reading them: 8192 x 8
+// rows of 2048 bf16 49 us (6.1 TB/s, part of it from the memory-side cache).
+template <typename T>
+__global__ void __launch_bounds__(kCombineThreads) combine_routes_kernel(const T* __restrict__ routes,
                                                                          const int32_t* __restrict__ ids, int num_rows,
                                                                          int shared, int M, int k, int H,
                                                                          uint16_t* __restrict__ y) {
@@ -31,10 +48,10 @@ __global__ void __launch_bounds__(kCombineThreads) combine_routes_kernel(const u
   if (i >= static_cast<long long>(M) * per) return;
   const int t = static_cast<int>(i / per), h = static_cast<int>(i % per) * 8;
   const int32_t* const tid = ids + static_cast<size_t>(t) * k;
-  const uint16_t* const first = routes + static_cast<size_t>(t) * k * H + h;
+  const T* const first = routes + static_cast<size_t>(t) * k * H + h;
   float acc[8] = {};
   for (int j0 = 0; j0 < k; j0 += 8) {
-    u32x4 v[8];
+    u32x4 v[8][sizeof(T) / 2];
     bool in[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -43,24 +60,15 @@ __global__ void __launch_bounds__(kCombineThreads) combine_routes_kernel(const u
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (in[j]) v[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(first + static_cast<size_t>(j0 + j) * H));
+      if (in[j]) load_row8(first + static_cast<size_t>(j0 + j) * H, v[j]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (!in[j]) continue;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        acc[2 * w] += __uint_as_float(v[j][w] << 16);
-        acc[2 * w + 1] += __uint_as_float(v[j][w] & 0xffff0000u);
-      }
-    }
+    for (int j = 0; j < 8; ++j)
+      if (in[j]) add_row8<T>(acc, v[j]);
   }
   if (shared) {
-    const u32x4 v = *reinterpret_cast<const u32x4*>(routes + (static_cast<size_t>(M) * k + t) * H + h);
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      acc[2 * w] += __uint_as_float(v[w] << 16);
-      acc[2 * w + 1] += __uint_as_float(v[w] & 0xffff0000u);
-    }
+    u32x4 v[sizeof(T) / 2];
+    load_row8(routes + (static_cast<size_t>(M) * k + t) * H + h, v);
+    add_row8<T>(acc, v);
   }
   u32x4 o;
 #pragma unroll
@@ -145,12 +153,16 @@ hipError_t launch_matmul(const MatmulArgs& a, hipStream_t stream) {
   return launch_matmul_tile(a, best->shape, best->shape == kTile256x128 && a.E > 1 && rows <= 64ll * a.E, stream);
 }
 
-hipError_t launch_combine_routes(const uint16_t* routes, const int32_t* ids, int num_rows, bool shared, int M,
+hipError_t launch_combine_routes(const void* routes, bool f32, const int32_t* ids, int num_rows, bool shared, int M,
                                  int k, int H, uint16_t* y, hipStream_t stream) {
   const long long n = static_cast<long long>(M) * (H / 8);
-  hipLaunchKernelGGL(combine_routes_kernel,
-                     dim3(static_cast<unsigned>((n + kCombineThreads - 1) / kCombineThreads)), dim3(kCombineThreads), 0,
-                     stream, routes, ids, num_rows, static_cast<int>(shared), M, k, H, y);
+  const dim3 grid(static_cast<unsigned>((n + kCombineThreads - 1) / kCombineThreads)), block(kCombineThreads);
+  if (f32)
+    hipLaunchKernelGGL(combine_routes_kernel<float>, grid, block, 0, stream, static_cast<const float*>(routes), ids,
+                       num_rows, static_cast<int>(shared), M, k, H, y);
+  else
+    hipLaunchKernelGGL(combine_routes_kernel<uint16_t>, grid, block, 0, stream, static_cast<const uint16_t*>(routes),
+                       ids, num_rows, static_cast<int>(shared), M, k, H, y);
   return hipGetLastError();
 }
 

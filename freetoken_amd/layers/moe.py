@@ -133,7 +133,7 @@ class MoELayer:
         assert not self.apply_router_weight_on_input or self.weight_format == "bf16"
         if self.weight_format == "int8":  # one path for both phases
             return ops.experts_int8(hidden_states, topk_weights, topk_ids, self.bank(), shared=self.shared_expert,
-                                    activation=self.activation)
+                                    activation=self.activation, route_dtype=torch.float32)
         fn = ops.experts_prefill if prefill else ops.experts_decode
         return fn(hidden_states, topk_weights, topk_ids, self.bank(), shared=self.shared_expert,
                   activation=self.activation)

@@ -738,11 +738,14 @@ def quantize_bank_int8(bank: ExpertBank) -> ExpertBank:
 
 def experts_int8(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.Tensor, bank: ExpertBank,
                  shared: ExpertBank | None = None, activation: str = "silu",
-                 out: torch.Tensor | None = None) -> torch.Tensor:
+                 out: torch.Tensor | None = None, route_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """Experts of an int8 bank (+ optional int8 shared expert) for a precomputed
     routing, decode and prefill alike: 8-bit products with one scale per token
     (per route between the two products) and per output channel (see
-    ftmoe_experts_int8).  Ids outside the bank's rows are skipped."""
+    ftmoe_experts_int8).  Ids outside the bank's rows are skipped.  A token's
+    weighted rows, one per route, are summed in float32 from rows of
+    ``route_dtype``: bfloat16, as in the other expert calls, or float32, where
+    nothing but the result is rounded, for twice the bytes of these rows."""
     if x.dtype != torch.bfloat16:
         raise ValueError("hidden_states must be bfloat16")
     if topk_w.dtype != torch.float32 or topk_ids.dtype != torch.int32:
@@ -753,6 +756,8 @@ def experts_int8(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.Tensor, 
         raise ValueError(f"Unsupported activation: {activation}")
     if bank.fmt != "int8" or (shared is not None and shared.fmt != "int8"):
         raise ValueError("experts_int8 takes int8 banks")
+    if route_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("the routes' rows are bfloat16 or float32")
     dev = _one_gpu(x, topk_w, topk_ids, out, bank.gate_up, bank.down, bank.gate_up_scale, bank.down_scale,
                    *((shared.gate_up, shared.down, shared.gate_up_scale, shared.down_scale) if shared else ()))
     m, k = topk_ids.shape
@@ -767,10 +772,11 @@ def experts_int8(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.Tensor, 
     bp = ctypes.byref(b)
     sp = ctypes.byref(sb) if sb is not None else None
     # a workspace of the call's own: of the stream's pool, or of the graph's under capture
-    ws = torch.empty((lib().ftmoe_experts_int8_workspace(m, k, bp, sp),), dtype=torch.uint8, device=dev)
+    rows = _lib.DTYPE_F32 if route_dtype == torch.float32 else _lib.DTYPE_BF16
+    ws = torch.empty((lib().ftmoe_experts_int8_rows_workspace(m, k, bp, sp, rows),), dtype=torch.uint8, device=dev)
     y = out if out is not None else torch.empty_like(x)
-    _launch("experts_int8", lib().ftmoe_experts_int8, dev, _ptr(x), m, k, _ptr(topk_w), _ptr(topk_ids), bp, sp,
-            _lib.ACT[activation], _ptr(y), _ptr(ws), ws.numel())
+    _launch("experts_int8", lib().ftmoe_experts_int8_rows, dev, _ptr(x), m, k, _ptr(topk_w), _ptr(topk_ids), bp, sp,
+            _lib.ACT[activation], rows, _ptr(y), _ptr(ws), ws.numel())
     return y
 
 

@@ -1,0 +1,125 @@
+"""Numerics of the int8 products and the int8 expert layer at their edges, against
+64 bits.
+
+Roundings: to float32 at most 2^-24 of the value, to bf16 2^-8.  A product's row is
+an exact integer converted to float32 and multiplied by its factors: five roundings
+at most, below 2^-21.  A sum of n float32 values in order is off by at most n 2^-24
+of the sum of their magnitudes.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from freetoken_amd import ops
+from freetoken_amd.layers.moe import MoELayer
+
+from test_gpu_int8 import BF16, F32, gen, int8_rows, make_bank, routing, scales, within
+
+pytestmark = pytest.mark.gpu
+
+
+def activations(x, ids, bank, act="silu"):
+    """Codes and scales of the routes' activations between the two products, from the operators one by one."""
+    M, k = ids.shape
+    q, s = ops.act_quant_int8(x)
+    order, offsets = ops.group_routes(ids, bank.num_rows)
+    h = torch.zeros((M * k, bank.inter), dtype=torch.bfloat16, device=x.device)
+    ops.grouped_matmul(q, bank.gate_up, offsets, order=order, top_k=k, x_scale=s, w_scale=bank.gate_up_scale,
+                       activation=act, out=h)
+    return ops.act_quant_int8(h)
+
+
+def down_rows(hq, hs, ids, bank, tw):
+    """The routes' weighted rows in 64 bits, [M, k, H]; zeros where a route has no expert."""
+    flat = ids.view(-1)
+    rows = torch.zeros((flat.numel(), bank.hidden), dtype=torch.float64, device=hq.device)
+    for e in range(bank.num_rows):
+        at = torch.nonzero(flat == e)[:, 0]
+        if at.numel():
+            rows[at] = (hq[at].double() @ bank.down[e].double().T) * hs[at].double()[:, None] * bank.down_scale[e].double()
+    return (rows * tw.double().view(-1, 1)).view(*ids.shape, -1)
+
+
+@pytest.mark.parametrize("M,k,E,H,I,Is", [(1, 2, 16, 1024, 512, 0), (1, 8, 128, 2048, 768, 768), (3, 9, 12, 272, 144, 48),
+                                          (40, 4, 8, 2064, 400, 400), (300, 8, 16, 640, 384, 16),
+                                          (1500, 6, 16, 512, 256, 256)])
+def test_float32_rows_are_rounded_once(dev, M, k, E, H, I, Is):
+    """With float32 rows nothing between the down products and the result is rounded to fewer bits: the error is that
+    of one rounding to bf16, however far the routes cancel."""
+    g = gen(dev, M + H)
+    bank, shared = make_bank(dev, g, E, H, I), make_bank(dev, g, 1, H, Is) if Is else None
+    x = torch.randn((M, H), generator=g, device=dev).to(torch.bfloat16)
+    tw, ids = routing(dev, g, M, k, E)
+    if M > 2:
+        ids[1::3] = -1
+        ids[0, 0] = E
+    y = ops.experts_int8(x, tw, ids, bank, shared=shared, route_dtype=torch.float32)
+    rows = down_rows(*activations(x, ids, bank), ids, bank, tw)
+    if shared is not None:
+        one = torch.zeros((M, 1), dtype=torch.int32, device=dev)
+        rows = torch.cat([rows, down_rows(*activations(x, one, shared), one, shared, torch.ones((M, 1), device=dev))], 1)
+    ref, size = rows.sum(1), rows.abs().sum(1)
+    off = size * (F32 + (k + 1) * 2.0**-24)
+    within(y, ref, off + (ref.abs() + off) * BF16)
+    # (rows rounded to bf16 first are not within it)
+    y = ops.experts_int8(x, tw, ids, bank, shared=shared)
+    assert not bool(((y.double() - ref).abs() <= off + (ref.abs() + off) * BF16).all())
+
+
+def test_layer_module_keeps_float32_rows(dev):
+    """MoELayer sums the routes from float32 rows, in small steps and batches, with a shared expert and without."""
+    g = gen(dev, 31)
+    E, H, I, k = 16, 512, 256, 4
+    bank, shared = make_bank(dev, g, E, H, I), make_bank(dev, g, 1, H, I)
+    layer = MoELayer(E, k, H, I, weight_format="int8", device=dev)
+    for name in ("gate_up", "down"):
+        getattr(layer, name + "_proj").copy_(getattr(bank, name))
+        getattr(layer, name + "_scale").copy_(getattr(bank, name + "_scale"))
+    for M in (1, 7, 500):
+        x = torch.randn((M, H), generator=g, device=dev).to(torch.bfloat16)
+        tw, ids = routing(dev, g, M, k, E)
+        for layer.shared_expert in (None, shared):
+            want = ops.experts_int8(x, tw, ids, bank, shared=layer.shared_expert, route_dtype=torch.float32)
+            assert torch.equal(layer.routed_forward(x, tw, ids), want)
+
+
+def test_float32_rows_do_not_depend_on_the_batch(dev):
+    g = gen(dev, 32)
+    E, H, I, k = 128, 2048, 768, 8
+    bank, shared = make_bank(dev, g, E, H, I), make_bank(dev, g, 1, H, I)
+    x = torch.randn((600, H), generator=g, device=dev).to(torch.bfloat16)
+    tw, ids = routing(dev, g, 600, k, E)
+    whole = ops.experts_int8(x, tw, ids, bank, shared=shared, route_dtype=torch.float32)
+    for first, n in [(0, 1), (1, 2), (7, 4), (64, 40), (300, 299)]:
+        part = slice(first, first + n)
+        y = ops.experts_int8(x[part], tw[part], ids[part], bank, shared=shared, route_dtype=torch.float32)
+        assert torch.equal(y, whole[part]), n
+
+
+@pytest.mark.parametrize("M", [2, 200])
+def test_float32_rows_in_a_replayed_graph(dev, M):
+    """A captured layer replayed with new inputs, eager calls in between."""
+    g = gen(dev, M)
+    E, H, I, k = 32, 512, 256, 4
+    bank, shared = make_bank(dev, g, E, H, I), make_bank(dev, g, 1, H, I)
+
+    def inputs():
+        return (torch.randn((M, H), generator=g, device=dev).to(torch.bfloat16), *routing(dev, g, M, k, E))
+
+    def step(x, tw, ids):
+        return ops.experts_int8(x, tw, ids, bank, shared=shared, route_dtype=torch.float32)
+
+    step(*inputs())
+    torch.cuda.synchronize()
+    bufs, graph = inputs(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*bufs)
+    for _ in range(3):
+        for b, v in zip(bufs, inputs()):
+            b.copy_(v)
+        want = step(*[b.clone() for b in bufs])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
