@@ -292,7 +292,7 @@ def _own_run(c, s):
     if s["shared"] is not None:
         gate_up, gs, down, ds = s["shared"]
         shared = ops.ExpertBank("int8", gate_up, down, gs, ds)
-    return ops.experts_int8(s["x"], s["tw"], s["ids"], bank, shared=shared)
+    return ops.experts_int8(s["x"], s["tw"], s["ids"], bank, shared=shared, route_dtype=torch.float32)
 
 
 def run(state):
