@@ -50,6 +50,14 @@ __device__ __forceinline__ typename Acc32<INT8>::type mma32(u32x4 a, u32x4 b, ty
 // silu by the reciprocal instruction (off by about 2^-23), as every form takes it.
 __device__ __forceinline__ float silu_of(float g) { return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g)); }
 
+// swiglu_clamp that keeps a NaN (minima and maxima drop it): a row of NaN stays one.
+__device__ __forceinline__ void clamp_numbers(float lim, float& g, float& u) {
+  if (lim > 0.f) {
+    g = g > lim ? lim : g;
+    u = u > lim ? lim : u < -lim ? -lim : u;
+  }
+}
+
 // Rows [begin, end) of group e in the grouped order, cut to [0, rows] whatever
 // the offsets hold; group E is the extra one.
 __device__ __forceinline__ void group_range(const MatmulArgs& a, int e, int& begin, int& end) {

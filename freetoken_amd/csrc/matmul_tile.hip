@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(kWave* WR* WC) matmul_tile_kernel(MatmulArgs a
               if constexpr (plain.value) {
                 y = silu_of(y) * u;
               } else {
-                swiglu_clamp(limit, y, u);
+                clamp_numbers(limit, y, u);
                 y = (a.act == ACT_SILU ? silu_of(y) : act_apply(a.act, y)) * u;
               }
             }

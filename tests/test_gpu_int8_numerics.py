@@ -123,3 +123,47 @@ def test_float32_rows_in_a_replayed_graph(dev, M):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("shared", [False, True], ids=["routed", "shared"])
+@pytest.mark.parametrize("M,H,I", [(3, 512, 256), (4, 2048, 768), (6, 2064, 528), (90, 512, 384), (400, 1024, 512)])
+def test_clamped_swiglu_keeps_nan(dev, M, H, I, shared):
+    """With a limit too, a token with an infinity or a NaN is NaN in its own row alone, whatever the step's size."""
+    g = gen(dev, M + H)
+    E, k = 24, 4
+    bank, sb = make_bank(dev, g, E, H, I), make_bank(dev, g, 1, H, I) if shared else None
+    for b in (bank, sb) if shared else (bank,):
+        b.swiglu_limit = 0.75
+    x = torch.randn((M, H), generator=g, device=dev).to(torch.bfloat16)
+    tw, ids = routing(dev, g, M, k, E)
+    fine = ops.experts_int8(x, tw, ids, bank, shared=sb)
+    assert bool(torch.isfinite(fine).all())
+    x[1, 5], x[2, 0] = float("nan"), float("-inf")
+    y = ops.experts_int8(x, tw, ids, bank, shared=sb)
+    assert bool(torch.isnan(y[1:3]).all())
+    keep = [i for i in range(M) if i not in (1, 2)]
+    assert torch.equal(y[keep], fine[keep])
+
+
+def test_clamped_swiglu_of_finite_values(dev):
+    """The clamp at its borders: gates and ups beyond, at and within the limit, and infinite products of finite rows."""
+    H = I = 16
+    one, more = torch.ones((1, 2 * I), device=dev), torch.ones((1, H), device=dev)
+    bank = ops.ExpertBank("int8", torch.zeros((1, 2 * I, H), dtype=torch.int8, device=dev),
+                          torch.zeros((1, H, I), dtype=torch.int8, device=dev), one, more, swiglu_limit=2.0)
+    bank.gate_up[0, :I, 0] = torch.tensor([0, 1, -1, 2, 3, 127, -127, 4, 2, 2, 2, 2, 2, 2, 2, 2], device=dev)
+    bank.gate_up[0, I:, 0] = torch.tensor([5, 1, -1, 2, -2, 3, -3, 127, -127, 2, 0, 1, 4, -4, 1, 1], device=dev)
+    bank.gate_up_scale[0, 14] = float("inf")  # an infinite gate is capped, an infinite up clamped
+    bank.gate_up_scale[0, I + 15] = float("inf")
+    bank.down[0, torch.arange(I), torch.arange(I)] = 127
+    for M in (1, 40, 400):
+        x = torch.zeros((M, H), dtype=torch.bfloat16, device=dev)
+        x[:, 0] = 1.0  # codes 127 of 1/127: one
+        ids = torch.zeros((M, 1), dtype=torch.int32, device=dev)
+        tw = torch.ones((M, 1), device=dev)
+        y = ops.experts_int8(x, tw, ids, bank, route_dtype=torch.float32)
+        h = (bank.gate_up[0, :, 0].double() * bank.gate_up_scale[0].double()).clamp(max=1e30)
+        gate, up = h[:I].clamp(max=2.0), h[I:].clamp(-2.0, 2.0)
+        a = (gate * torch.sigmoid(gate) * up).to(torch.bfloat16).double()
+        want = (127 * a / a.abs().max()).round() * a.abs().max()
+        within(y, want.expand(M, -1), want.abs() * (BF16 + F32))
