@@ -47,9 +47,6 @@ __device__ __forceinline__ typename Acc32<INT8>::type mma32(u32x4 a, u32x4 b, ty
                                                    0);
 }
 
-// silu by the reciprocal instruction (off by about 2^-23), as every form takes it.
-__device__ __forceinline__ float silu_of(float g) { return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g)); }
-
 // swiglu_clamp that keeps a NaN (minima and maxima drop it): a row of NaN stays one.
 __device__ __forceinline__ void clamp_numbers(float lim, float& g, float& u) {
   if (lim > 0.f) {

@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(W* kWave) matmul_stream_kernel(MatmulArgs a) {
           float u = static_cast<float>(su[v]);
           if (INT8) u *= ws[n_out + f] * xs;
           clamp_numbers(limit, y, u);
-          y = (a.act == ACT_SILU ? silu_of(y) : act_apply(a.act, y)) * u;
+          y = act_apply(a.act, y) * u;
         }
         o[v] = INT8 && !GATE ? y : y * wt;
       }

@@ -296,10 +296,10 @@ __global__ void __launch_bounds__(kWave* WR* WC) matmul_tile_kernel(MatmulArgs a
               float u = static_cast<float>(acc[RT / 2 + j][i][4 * q + v]);
               if (INT8) u *= ws[RT / 2 + j][q][v] * xs;
               if constexpr (plain.value) {
-                y = silu_of(y) * u;
+                y = act_apply(ACT_SILU, y) * u;
               } else {
                 clamp_numbers(limit, y, u);
-                y = (a.act == ACT_SILU ? silu_of(y) : act_apply(a.act, y)) * u;
+                y = act_apply(a.act, y) * u;
               }
             }
             o[v] = INT8 && !GATE ? y : y * rw;

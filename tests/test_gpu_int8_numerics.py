@@ -167,3 +167,22 @@ def test_clamped_swiglu_of_finite_values(dev):
         a = (gate * torch.sigmoid(gate) * up).to(torch.bfloat16).double()
         want = (127 * a / a.abs().max()).round() * a.abs().max()
         within(y, want.expand(M, -1), want.abs() * (BF16 + F32))
+
+
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("M", [1, 40, 300])
+def test_silu_relative_to_its_result(dev, M, out_dtype):
+    """silu(gate) up over gates from -88 to 88, the smallest results among normal numbers, relative to the result: the
+    exponential of x is off by about |x| 2^-24 and 2^-22 relative, the other operations by 2^-21 together: below 2^-16."""
+    g = gen(dev, M)
+    K, n = 16, 1760
+    gate = (torch.arange(n, device=dev) - n / 2 + 0.5).mul_(0.1)
+    q = torch.zeros((M, K), dtype=torch.int8, device=dev)
+    q[:, 0] = 1
+    w = torch.zeros((2 * n, K), dtype=torch.int8, device=dev)
+    w[:, 0] = 1
+    ws = torch.cat([gate, torch.rand(n, generator=g, device=dev) + 1.0])  # (a channel's scale may be any number)
+    y = ops.matmul_int8(q, torch.ones(M, device=dev), w, ws, activation="silu", out_dtype=out_dtype)
+    ref = (gate.double() * torch.sigmoid(gate.double()) * ws[n:].double()).expand(M, -1)
+    assert float(ref.abs().min()) > 2.0**-126
+    within(y, ref, ref.abs() * (2.0**-16 + (BF16 if out_dtype == torch.bfloat16 else 0)))
