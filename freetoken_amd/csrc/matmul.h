@@ -47,6 +47,18 @@ __device__ __forceinline__ typename Acc32<INT8>::type mma32(u32x4 a, u32x4 b, ty
                                                    0);
 }
 
+// An exact integer sum times its row's and its channel's scale, in an order that leaves the range of normal numbers
+// only where the result does: a sum is 0 or at least 1 in magnitude, so the row's scale comes first where it is
+// below 1 (the channel's may be large) and last where it is not (the channel's may be small).  One of the two parts
+// is 1, so that there are two roundings; every form multiplies in this order.
+struct RowFactor {
+  float first, last;
+};
+__device__ __forceinline__ RowFactor row_factor(float scale) {
+  return scale < 1.0f ? RowFactor{scale, 1.0f} : RowFactor{1.0f, scale};
+}
+__device__ __forceinline__ float scaled(float sum, const RowFactor& x, float ws) { return sum * x.first * ws * x.last; }
+
 // swiglu_clamp that keeps a NaN (minima and maxima drop it): a row of NaN stays one.
 __device__ __forceinline__ void clamp_numbers(float lim, float& g, float& u) {
   if (lim > 0.f) {

@@ -299,20 +299,20 @@ __global__ void __launch_bounds__(W* kWave) matmul_stream_kernel(MatmulArgs a) {
       const acc_t su = GATE ? sum(NJ + j, c) : sg;
       const float xs = QX ? s_xs[16 * c + r16] : INT8 ? a.xs[x_row(r)] : 1.0f;
       const float wt = a.row_weight && r < a.rows ? a.row_weight[r] : 1.0f;
-      const float by = GATE ? xs : xs * wt;  // (the same products in every form)
+      const RowFactor rf = row_factor(xs);
       float o[4];
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         const int f = min(nn + v, n_out - 1);
         float y = static_cast<float>(sg[v]);
-        if (INT8) y *= ws[f] * by;
+        if (INT8) y = scaled(y, rf, ws[f]);
         if constexpr (GATE) {
           float u = static_cast<float>(su[v]);
-          if (INT8) u *= ws[n_out + f] * xs;
+          if (INT8) u = scaled(u, rf, ws[n_out + f]);
           clamp_numbers(limit, y, u);
           y = act_apply(a.act, y) * u;
         }
-        o[v] = INT8 && !GATE ? y : y * wt;
+        o[v] = y * wt;
       }
       const size_t at = static_cast<size_t>(r) * n_out + nn;
       if (n_out % 4 == 0) {

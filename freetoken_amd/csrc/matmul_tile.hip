@@ -9,7 +9,7 @@
 //
 // int8 sums stay int32 to the end (exact), bf16 ones float32; a result is the sum
 // times its channel's and its row's scale (and weight), rounded to bf16 once; the
-// factors are multiplied in the order of the streaming form.
+// factors are multiplied as in the streaming form (matmul.h: scaled).
 //
 // Two waves per SIMD and 32 x 32 MFMAs: one wave with 16 x 16 ones issues 2930 int8
 // T/s at most, two 4000, one with 32 x 32 ones 4100 (8192 x 4096 x 7168: 227 us with 4
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(kWave* WR* WC) matmul_tile_kernel(MatmulArgs a
       const int col = 32 * CT * wc + 32 * i + r32;
       const float xs = INT8 ? s_xs(b)[col] : 1.0f;
       const float rw = a.row_weight ? s_rw(b)[col] : 1.0f;
-      const float by = GATE ? xs : xs * rw;
+      const RowFactor rf = row_factor(xs);
       const int r = out_f32 ? route_of(t, b, col) : 0;
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
@@ -291,10 +291,10 @@ __global__ void __launch_bounds__(kWave* WR* WC) matmul_tile_kernel(MatmulArgs a
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             float y = static_cast<float>(acc[j][i][4 * q + v]);
-            if (INT8) y *= ws[j][q][v] * by;
+            if (INT8) y = scaled(y, rf, ws[j][q][v]);
             if constexpr (GATE) {
               float u = static_cast<float>(acc[RT / 2 + j][i][4 * q + v]);
-              if (INT8) u *= ws[RT / 2 + j][q][v] * xs;
+              if (INT8) u = scaled(u, rf, ws[RT / 2 + j][q][v]);
               if constexpr (plain.value) {
                 y = act_apply(ACT_SILU, y) * u;
               } else {
@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(kWave* WR* WC) matmul_tile_kernel(MatmulArgs a
                 y = act_apply(a.act, y) * u;
               }
             }
-            o[v] = INT8 && !GATE ? y : y * rw;
+            o[v] = y * rw;
           }
           if (!out_f32) {
             const int chunk = (4 * j + q) ^ (r32 & (NC - 1));

@@ -186,3 +186,35 @@ def test_silu_relative_to_its_result(dev, M, out_dtype):
     ref = (gate.double() * torch.sigmoid(gate.double()) * ws[n:].double()).expand(M, -1)
     assert float(ref.abs().min()) > 2.0**-126
     within(y, ref, ref.abs() * (2.0**-16 + (BF16 if out_dtype == torch.bfloat16 else 0)))
+
+
+# (largest magnitudes of the rows, of the weights), so that a product of scales leaves the normal numbers on the way
+FAR = [(2.0**-117, 2.0**-4), (2.0**-120, 2.0**-3), (2.0**-60, 2.0**-62), (2.0**126, 2.0**-110), (2.0**127, 2.0**-126),
+       (2.0**-126, 2.0**120), (2.0**64, 2.0**50), (2.0**100, 2.0**-40)]
+
+
+@pytest.mark.parametrize("top,wtop", FAR, ids=range(len(FAR)))
+@pytest.mark.parametrize("M", [1, 40, 300])
+def test_far_scales(dev, M, top, wtop):
+    """Rows and weights far from 1: the exact sum times its factors, right wherever the result and each scale are
+    normal float32 numbers; a sum of zero is zero."""
+    g = gen(dev, M)
+    N, K = 200, 272
+    x = torch.randint(-128, 129, (M, K), generator=g, device=dev).double().mul_(2.0**-8)
+    x[:, 3] = 1.0
+    q, s = ops.act_quant_int8((x * top).to(torch.bfloat16))
+    w, ws = int8_rows(dev, g, N, K), (torch.rand(N, generator=g, device=dev) + 1.0).mul_(wtop / 254)
+    w[7] = 0
+    sums = q.double() @ w.double().T
+    ref = sums * s.double()[:, None] * ws.double()
+    # scales below the normal numbers hold fewer bits themselves, and are compared as they are
+    normal = (ref.abs() >= 2.0**-126) & (ref.abs() < 2.0**127) | (sums == 0)
+    assert int(normal.sum()) >= normal.numel() // 2
+    y = ops.matmul_int8(q, s, w, ws, out_dtype=torch.float32)
+    within(torch.where(normal, y.double(), 0.0), torch.where(normal, ref, 0.0), ref.abs() * F32)
+    offsets = torch.tensor([0, M], dtype=torch.int32, device=dev)
+    weight = torch.rand(M, generator=g, device=dev)
+    y = ops.grouped_matmul(q, w[None], offsets, x_scale=s, w_scale=ws[None], row_weight=weight)
+    ref = ref * weight.double()[:, None]
+    normal &= (ref.abs() >= 2.0**-126) | (sums == 0)
+    within(torch.where(normal, y.double(), 0.0), torch.where(normal, ref, 0.0), ref.abs() * (F32 + BF16))
