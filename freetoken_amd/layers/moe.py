@@ -14,7 +14,7 @@ Differences from the reference, all additive:
     converts exactly);
   * ``swiglu_limit`` (set through ``make_moe_layer``'s ``extra_attrs``, as the
     reference's engine does) clamps the SwiGLU of the ds_fp4 experts in both
-    regimes (``layers/moe.py:473,550-573``).
+    regimes (``layers/moe.py:473,550-573``), and of the int8 ones.
 TP is 1 (one GPU): ``_maybe_all_reduce`` is the identity.
 """
 
@@ -28,6 +28,7 @@ from .. import ops
 from ..core import get_global_ctx, has_global_ctx
 from ..moe import is_offload_moe_backend
 from ..moe.fused import GROUPED_MIN_ROUTES, fused_experts_impl, fused_topk
+from ..moe.fused_int8 import fused_experts_int8
 from ..moe.offload_cache import bank_from_views
 
 if TYPE_CHECKING:
@@ -132,8 +133,9 @@ class MoELayer:
                                       apply_router_weight_on_input=self.apply_router_weight_on_input)
         assert not self.apply_router_weight_on_input or self.weight_format == "bf16"
         if self.weight_format == "int8":  # one path for both phases
-            return ops.experts_int8(hidden_states, topk_weights, topk_ids, self.bank(), shared=self.shared_expert,
-                                    activation=self.activation, route_dtype=torch.float32)
+            return fused_experts_int8(hidden_states, self.gate_up_proj, self.gate_up_scale, self.down_proj,
+                                      self.down_scale, topk_weights, topk_ids, activation=self.activation,
+                                      shared=self.shared_expert, swiglu_limit=self.swiglu_limit)
         fn = ops.experts_prefill if prefill else ops.experts_decode
         return fn(hidden_states, topk_weights, topk_ids, self.bank(), shared=self.shared_expert,
                   activation=self.activation)

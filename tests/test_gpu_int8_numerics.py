@@ -14,6 +14,7 @@ import torch
 
 from freetoken_amd import ops
 from freetoken_amd.layers.moe import MoELayer
+from freetoken_amd.moe.fused_int8 import fused_experts_int8
 
 from test_gpu_int8 import BF16, F32, gen, int8_rows, make_bank, routing, scales, within
 
@@ -218,3 +219,37 @@ def test_far_scales(dev, M, top, wtop):
     ref = ref * weight.double()[:, None]
     normal &= (ref.abs() >= 2.0**-126) | (sums == 0)
     within(torch.where(normal, y.double(), 0.0), torch.where(normal, ref, 0.0), ref.abs() * (F32 + BF16))
+
+
+@pytest.mark.parametrize("M", [2, 300])
+def test_fused_experts_int8(dev, M):
+    """The functional form and MoELayer are ops.experts_int8 with float32 rows, the clamp of a model with clamped SwiGLU
+    among their arguments."""
+    g = gen(dev, M)
+    E, H, I, k = 16, 512, 256, 4
+    bank, shared = make_bank(dev, g, E, H, I), make_bank(dev, g, 1, H, I)
+    x = torch.randn((M, H), generator=g, device=dev).to(torch.bfloat16)
+    tw, ids = routing(dev, g, M, k, E)
+    layer = MoELayer(E, k, H, I, weight_format="int8", device=dev)
+    for name in ("gate_up", "down"):
+        getattr(layer, name + "_proj").copy_(getattr(bank, name))
+        getattr(layer, name + "_scale").copy_(getattr(bank, name + "_scale"))
+    arrays = (bank.gate_up, bank.gate_up_scale, bank.down, bank.down_scale)
+    results = []
+    for limit in (None, 0.0, 0.5):
+        for sb in (None, shared):
+            bank.swiglu_limit = limit or 0.0
+            want = ops.experts_int8(x, tw, ids, bank, shared=sb, route_dtype=torch.float32)
+            assert torch.equal(fused_experts_int8(x, *arrays, tw, ids, shared=sb, swiglu_limit=limit), want)
+            layer.swiglu_limit, layer.shared_expert = limit, sb
+            assert torch.equal(layer.routed_forward(x, tw, ids), want)
+            results.append(want)
+    assert torch.equal(results[0], results[2]) and not torch.equal(results[2], results[4])
+    assert torch.equal(fused_experts_int8(x, *arrays, tw, ids), results[0])
+    gelu = fused_experts_int8(x, *arrays, tw, ids, activation="gelu")
+    bank.swiglu_limit = 0.0
+    assert torch.equal(gelu, ops.experts_int8(x, tw, ids, bank, activation="gelu", route_dtype=torch.float32))
+    with pytest.raises(ValueError, match="silu"):
+        fused_experts_int8(x, *arrays, tw, ids, activation="gelu", swiglu_limit=0.5)
+    with pytest.raises(ValueError, match="swiglu_limit"):
+        fused_experts_int8(x, *arrays, tw, ids, swiglu_limit=float("nan"))
