@@ -801,14 +801,15 @@ int ftmoe_experts_prefill(const void* x, int M, int top_k, const float* topk_w, 
 namespace {
 
 constexpr int kInt8MaxK = 131056;  // 127 * 128 * K stays below 2^31
+constexpr int kProductMaxN = 1 << 30;  // features past the last one, in tiles, stay below 2^31
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 int check_product(const ftmoe::MatmulArgs& a, const char* what) {
   const int step = a.int8 ? 16 : 8, most = a.int8 ? kInt8MaxK : INT32_MAX / 4;
-  if (a.N <= 0 || a.K <= 0 || a.K % step || a.K > most)
-    return fail(FTMOE_ERR_UNSUPPORTED, "%s: N=%d K=%d (K a positive multiple of %d, at most %d)", what, a.N, a.K, step,
-                most);
+  if (a.N <= 0 || a.N > kProductMaxN || a.K <= 0 || a.K % step || a.K > most)
+    return fail(FTMOE_ERR_UNSUPPORTED, "%s: N=%d K=%d (N at most %d, K a positive multiple of %d, at most %d)", what, a.N,
+                a.K, kProductMaxN, step, most);
   if (a.act < FTMOE_ACT_NONE || a.act > FTMOE_ACT_GELU_TANH)
     return fail(FTMOE_ERR_UNSUPPORTED, "%s: activation %d", what, a.act);
   if (a.act != FTMOE_ACT_NONE && a.N % 2)

@@ -95,6 +95,7 @@ enum class Form { kTiles, kSplit, kWhole, kWide };
 Form form_of(const MatmulArgs& a) {
   const long long n_out = a.act < 0 ? a.N : a.N / 2, rows = a.rows, E = a.E;
   const long long tiles = (n_out + 15) / 16;  // of 16 features
+  if (tiles > 1 << 24) return Form::kTiles;   // a launch holds below 2^32 threads, 256 for 16 to 64 features when streaming
   if (E == 1) return rows <= 16 && tiles <= 384 ? Form::kSplit : rows <= 64 ? Form::kWide : Form::kTiles;
   if (rows > 4 * E) return rows <= 16 * E && tiles * E <= 1536 ? Form::kWide : Form::kTiles;
   // K is split where there are too few workgroups without it, or rows long enough for four streams

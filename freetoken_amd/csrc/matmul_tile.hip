@@ -194,7 +194,8 @@ __global__ void __launch_bounds__(kWave* WR* WC) matmul_tile_kernel(MatmulArgs a
     }
     if (INT8 && 64 * wave < ROWS) {
       const uint64_t ws = uniform_u64(reinterpret_cast<uint64_t>(extra ? a.extra_ws : a.ws) + first * 4);
-      lds_buf4(make_rsrc(reinterpret_cast<const void*>(ws), uniform((a.N - n0) * 4)),
+      // (N below 2^27 with gate and up rows: check_product)
+      lds_buf4(make_rsrc(reinterpret_cast<const void*>(ws), uniform((GATE ? a.N - n0 : min(a.N - n0, ROWS)) * 4)),
                reinterpret_cast<uint8_t*>(s_ws(b) + 64 * wave), static_cast<uint32_t>(trow_rel(64 * wave + ln)) * 4, 0);
     }
   };

@@ -354,7 +354,7 @@ int ftmoe_act_quant_int8(const void* x, int rows, int K, void* q, float* scales,
  * 32-bit integers: q int8 [M, K], w int8 [N, K], scales float32, y [M, N] of
  * out_dtype.  With an activation (not FTMOE_ACT_NONE) w holds N/2 gate rows,
  * then N/2 up rows, and y [M, N/2] = act(gate) * up of those products in
- * float32.  K <= 131056; x, and with an activation w, below 2 GiB. */
+ * float32.  K <= 131056, N <= 2^30; x, and with an activation w, below 2 GiB. */
 int ftmoe_matmul_int8(const void* q, const float* q_scale, const void* w, const float* w_scale, int M, int N, int K,
                       int activation, int out_dtype, void* y, ftmoe_stream_t stream);
 
@@ -371,7 +371,8 @@ int ftmoe_group_routes(const int32_t* topk_ids, int numel, int num_experts, int3
 /* Matrix products grouped by expert, each with a ragged set of rows:
  *   y[r] = row_weight[r] * (x[r / top_k] . w[e]^T)   for r = order[i] and offsets[e] <= i < offsets[e + 1],
  * with the sums in float32 (bf16) or exact in 32-bit integers and scaled (int8).
- * num_experts <= 1023; x, and with an activation each matrix, below 2 GiB. */
+ * num_experts <= 1023, N <= 2^30; x, 256 rows of w, and with an activation each
+ * matrix, below 2 GiB. */
 typedef struct ftmoe_grouped {
   int format;               /* FTMOE_FMT_BF16 or FTMOE_FMT_INT8: x and w */
   int num_experts, N, K;

@@ -253,3 +253,21 @@ def test_fused_experts_int8(dev, M):
         fused_experts_int8(x, *arrays, tw, ids, activation="gelu", swiglu_limit=0.5)
     with pytest.raises(ValueError, match="swiglu_limit"):
         fused_experts_int8(x, *arrays, tw, ids, swiglu_limit=float("nan"))
+
+
+def test_most_features(dev):
+    """As many output channels as a product takes: their scales and results past 2^31 bytes."""
+    g = gen(dev, 41)
+    K = 16
+    for N in (1 << 30, (1 << 29) + 24, (1 << 28) + 40):
+        q, s = int8_rows(dev, g, 2, K), scales(dev, g, 2)
+        w, ws = int8_rows(dev, g, N, K), scales(dev, g, N)
+        at = torch.cat([torch.arange(300, device=dev), torch.randint(0, N, (3000,), generator=g, device=dev),
+                        N - 1 - torch.arange(300, device=dev), (N // 2 + torch.arange(-150, 150, device=dev))])
+        ref = (q.double() @ w[at].double().T) * s.double()[:, None] * ws[at].double()
+        y = ops.matmul_int8(q, s, w, ws)
+        within(y[:, at], ref, ref.abs() * (F32 + BF16))
+        offsets = torch.tensor([0, 2], dtype=torch.int32, device=dev)
+        y = ops.grouped_matmul(q, w[None], offsets, x_scale=s, w_scale=ws[None])
+        within(y[:, at], ref, ref.abs() * (F32 + BF16))
+        del y, w, ws

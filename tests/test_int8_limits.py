@@ -34,3 +34,12 @@ def test_row_type_of_the_expert_layer():
     with pytest.raises(ValueError, match="rows are"):
         ops.experts_int8(torch.zeros((2, 32), dtype=torch.bfloat16), torch.ones((2, 1)),
                          torch.zeros((2, 1), dtype=torch.int32), b, route_dtype=torch.float16)
+
+
+def test_most_features():
+    L = _lib.lib()
+    n = (1 << 30) + 1
+    assert L.ftmoe_matmul_int8(P, P, P, P, 1, n, 16, -1, _lib.DTYPE_BF16, P, None) == UNSUPPORTED
+    for fmt in (_lib.FMT_INT8, _lib.FMT_BF16):
+        g = _lib.FtmoeGrouped(fmt, 1, n, 16, 4096, 4096, 4096, 4096, 1, 1, 4096, None, None, -1, 4096)
+        assert L.ftmoe_grouped_matmul(ctypes.byref(g), None) == UNSUPPORTED
