@@ -24,6 +24,7 @@ constexpr int kGroupWaves = 16;
 constexpr int kGroupThreads = kGroupWaves * kWave;
 constexpr int kGroupChunks = 2;  // 64-route chunks of a wave
 constexpr int kGroupRoutes = kGroupThreads * kGroupChunks;
+constexpr int kGroupQuantRows = 1 << 23;  // (four waves each: 2^31 threads, half of what a launch holds)
 
 struct GroupShared {
   uint16_t count[kGroupWaves][kCountMaxRows + 1];  // per wave and id, then the place of the wave's next route of it
@@ -192,9 +193,11 @@ size_t group_hist_ints(int numel, int num_experts) {
 
 hipError_t launch_group_routes(const GroupArgs& a, int32_t* hist, hipStream_t stream) {
   if (!a.x) return launch_group<0>(a, hist, stream);
-  if (a.K <= 2048) return launch_group<1>(a, hist, stream);
-  if (a.K <= 8192) return launch_group<4>(a, hist, stream);
-  // rows longer than a workgroup's registers: the quantisation in its own launch
+  if (a.x_rows <= kGroupQuantRows) {
+    if (a.K <= 2048) return launch_group<1>(a, hist, stream);
+    if (a.K <= 8192) return launch_group<4>(a, hist, stream);
+  }
+  // rows longer than a workgroup's registers, or too many for one launch: the quantisation in its own
   const hipError_t err = launch_act_quant_int8(a.x, a.x_rows, a.K, a.q, a.scales, stream);
   return err == hipSuccess ? launch_group<0>(a, hist, stream) : err;
 }

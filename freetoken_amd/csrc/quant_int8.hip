@@ -5,6 +5,8 @@
 // (5.7), one row of 7168 2.2 us.  Rows up to 2048 values take a wave, up to 8192 a
 // workgroup of four: all of a row's loads are in flight together and its values
 // stay in registers between the maximum and the codes.
+#include <algorithm>
+
 #include "quant_int8.h"
 
 namespace ftmoe {
@@ -26,13 +28,20 @@ __global__ void __launch_bounds__(kQuantThreads) act_quant_int8_kernel(const uin
 }  // namespace
 
 hipError_t launch_act_quant_int8(const uint16_t* x, int rows, int K, int8_t* q, float* scales, hipStream_t stream) {
-  const dim3 block(kQuantThreads);
-  if (K <= 2048)
-    hipLaunchKernelGGL((act_quant_int8_kernel<1, 4>), dim3((rows + 3) / 4), block, 0, stream, x, rows, K, q, scales);
-  else if (K <= 8192)
-    hipLaunchKernelGGL((act_quant_int8_kernel<4, 4>), dim3(rows), block, 0, stream, x, rows, K, q, scales);
-  else
-    hipLaunchKernelGGL((act_quant_int8_kernel<4, 0>), dim3(rows), block, 0, stream, x, rows, K, q, scales);
+  constexpr int kMost = 1 << 23;  // rows of a launch, which holds below 2^32 threads
+  for (long long first = 0; first < rows; first += kMost) {
+    const int n = static_cast<int>(std::min<long long>(kMost, rows - first));
+    const uint16_t* const xr = x + first * K;
+    int8_t* const qr = q + first * K;
+    float* const sr = scales + first;
+    const dim3 block(kQuantThreads);
+    if (K <= 2048)
+      hipLaunchKernelGGL((act_quant_int8_kernel<1, 4>), dim3((n + 3) / 4), block, 0, stream, xr, n, K, qr, sr);
+    else if (K <= 8192)
+      hipLaunchKernelGGL((act_quant_int8_kernel<4, 4>), dim3(n), block, 0, stream, xr, n, K, qr, sr);
+    else
+      hipLaunchKernelGGL((act_quant_int8_kernel<4, 0>), dim3(n), block, 0, stream, xr, n, K, qr, sr);
+  }
   return hipGetLastError();
 }
 

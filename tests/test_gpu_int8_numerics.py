@@ -271,3 +271,30 @@ def test_most_features(dev):
         y = ops.grouped_matmul(q, w[None], offsets, x_scale=s, w_scale=ws[None])
         within(y[:, at], ref, ref.abs() * (F32 + BF16))
         del y, w, ws
+
+
+@pytest.mark.parametrize("rows,K", [((1 << 26) + 5, 16), ((1 << 24) + 3, 2064)])
+def test_quant_more_rows_than_a_launch(dev, rows, K):
+    """More rows than one launch has threads for: the codes and scales of the rows alone."""
+    x = torch.empty((rows, K), dtype=torch.bfloat16, device=dev).normal_(generator=gen(dev, K))
+    q, s = ops.act_quant_int8(x)
+    for first in (0, (1 << 23) - 50, (1 << 24) - 50, rows - 100):
+        part = slice(max(0, first), min(rows, first + 100))
+        qp, sp = ops.act_quant_int8(x[part])
+        assert torch.equal(q[part], qp) and torch.equal(s[part], sp)
+    top = torch.stack([x[i : i + (1 << 22)].abs().amax(1).float().sum(dtype=torch.float64) for i in range(0, rows, 1 << 22)])
+    assert abs(float(s.sum(dtype=torch.float64) * 127 / top.sum()) - 1) < 1e-6
+
+
+def test_layer_of_more_tokens_than_a_launch(dev):
+    """An expert layer of more (short) tokens than the grouping's launch can quantise beside it."""
+    M, H, I, E = (1 << 24) + 7, 16, 16, 3
+    g = gen(dev, 51)
+    bank = make_bank(dev, g, E, H, I)
+    x = torch.empty((M, H), dtype=torch.bfloat16, device=dev).normal_(generator=g)
+    ids = torch.randint(0, E, (M, 1), generator=g, device=dev, dtype=torch.int32)
+    tw = torch.rand((M, 1), generator=g, device=dev)
+    y = ops.experts_int8(x, tw, ids, bank, route_dtype=torch.float32)
+    for first in (0, (1 << 23) - 50, M - 100):
+        part = slice(first, first + 100)
+        assert torch.equal(y[part], ops.experts_int8(x[part], tw[part], ids[part], bank, route_dtype=torch.float32))
