@@ -7,7 +7,10 @@
 // count, and their first lane alone keeps the wave's count of that expert: no
 // atomics, and the stable order.  Up to 2048 routes one workgroup does all of it in
 // one launch; beyond, workgroups of 2048 routes count first, and in a second launch
-// each adds up the counts before its own and places its routes.
+// each adds up the counts before its own and places its routes.  That reads every
+// count in every workgroup, which grows with the square of the routes: past
+// kGroupCounts counts a launch between the two turns each expert's counts into
+// their running sums.
 //
 // Bound by latency: 32 routes 3.5 us, 512 (with 64 tokens of 7168 quantised) 4.7 us,
 // 32768 4.9 + 6.4 us, 65536 (with 8192 tokens of 2048, 50 MB) 12.6 + 8.7 us.
@@ -25,6 +28,16 @@ constexpr int kGroupThreads = kGroupWaves * kWave;
 constexpr int kGroupChunks = 2;  // 64-route chunks of a wave
 constexpr int kGroupRoutes = kGroupThreads * kGroupChunks;
 constexpr int kGroupQuantRows = 1 << 23;  // (four waves each: 2^31 threads, half of what a launch holds)
+
+// Counts of all workgroups that each of them still adds up itself.  us in all, itself / with sums from a launch between:
+// 65536 routes 128 experts 9.5 / 10.7, 1023 experts 21.0 / 14.6; 131072 routes 8 experts 7.5 / 9.7, 128 11.1 / 10.9, 1023
+// 32.6 / 15.2; 1048576 routes 8 experts 12.1 / 12.8, 128 38.5 / 17.5, 1023 213 / 31.
+constexpr int kGroupCounts = 8192;
+
+int group_blocks(int numel) { return numel / kGroupRoutes + (numel % kGroupRoutes ? 1 : 0); }
+
+// Whether the running sums come from a launch of their own, in one more row of counts.
+bool group_sums(int blocks, int num_experts) { return static_cast<long long>(blocks) * (num_experts + 1) > kGroupCounts; }
 
 struct GroupShared {
   uint16_t count[kGroupWaves][kCountMaxRows + 1];  // per wave and id, then the place of the wave's next route of it
@@ -55,9 +68,10 @@ __device__ __forceinline__ int group_scan(int v, GroupShared& s, int* total) {
 }
 
 // One workgroup's routes [first, first + kGroupRoutes).  hist: null, or [blocks][E + 1]
-// counts of every workgroup (this one is `block`).
+// counts of every workgroup (this one is `block`); summed: those of the workgroups before
+// it instead, and behind them a row of all routes' counts.
 __device__ __forceinline__ void group_block(const GroupArgs& a, int block, int blocks, const int32_t* hist,
-                                            GroupShared& s) {
+                                            bool summed, GroupShared& s) {
   const int tid = threadIdx.x, lane = lane_id(), wave = tid / kWave;
   const int ids = a.num_experts + 1;  // id num_experts has a place of its own behind the experts
   const int bits = 32 - __clz(a.num_experts);
@@ -85,7 +99,13 @@ __device__ __forceinline__ void group_block(const GroupArgs& a, int block, int b
     if (id[c] >= 0 && rank[c] == 0) s.count[wave][id[c]] += static_cast<uint16_t>(__popcll(same[c]));
   }
   __syncthreads();
-  if (hist) {  // (integer sums in LDS: the order does not matter)
+  if (hist && summed) {
+    for (int e = tid; e < ids; e += kGroupThreads) {
+      s.before[e] = hist[static_cast<size_t>(block) * ids + e];
+      s.sum[e] = hist[static_cast<size_t>(blocks) * ids + e];
+    }
+    __syncthreads();
+  } else if (hist) {  // (integer sums in LDS: the order does not matter)
     for (int i = tid; i < blocks * ids; i += kGroupThreads) {
       const int n = hist[i], b = i / ids, e = i - b * ids;
       if (!n) continue;
@@ -122,7 +142,8 @@ __device__ __forceinline__ void group_block(const GroupArgs& a, int block, int b
     // (the wave's reads above are issued before this write)
     if (rank[c] == 0) s.count[wave][id[c]] = static_cast<uint16_t>(at + __popcll(same[c]));
   }
-  for (int i = total + block * kGroupThreads + tid; i < a.numel; i += blocks * kGroupThreads) a.order[i] = a.numel;
+  for (long long i = static_cast<long long>(total) + block * kGroupThreads + tid; i < a.numel; i += blocks * kGroupThreads)
+    a.order[i] = a.numel;
 }
 
 // The quantisation of rows by the workgroups behind the grouping ones.
@@ -141,7 +162,7 @@ __global__ void __launch_bounds__(kGroupThreads) group_routes_kernel(GroupArgs a
   if constexpr (WPR > 0) {
     if (blockIdx.x > 0) return quant_block<WPR>(a, blockIdx.x - 1);
   }
-  group_block(a, 0, 1, nullptr, s);
+  group_block(a, 0, 1, nullptr, false, s);
 }
 
 template <int WPR>
@@ -163,14 +184,31 @@ __global__ void __launch_bounds__(kGroupThreads) group_count_kernel(GroupArgs a,
   for (int e = threadIdx.x; e < ids; e += kGroupThreads) hist[static_cast<size_t>(blockIdx.x) * ids + e] = bins[e];
 }
 
-__global__ void __launch_bounds__(kGroupThreads) group_place_kernel(GroupArgs a, int blocks, const int32_t* hist) {
+// Workgroup e: the counts of id e by workgroup become those of the workgroups before, all of them in row `blocks`.
+__global__ void __launch_bounds__(kGroupThreads) group_sum_kernel(int ids, int blocks, int32_t* hist) {
   __shared__ GroupShared s;
-  group_block(a, blockIdx.x, blocks, hist, s);
+  int before = 0;
+  for (int b0 = 0; b0 < blocks; b0 += kGroupThreads) {  // (every thread takes part in the barriers)
+    const int b = b0 + static_cast<int>(threadIdx.x);
+    int32_t* const at = hist + static_cast<size_t>(b) * ids + blockIdx.x;
+    int total;
+    const int sum = group_scan(b < blocks ? *at : 0, s, &total);
+    if (b < blocks) *at = before + sum;
+    before += total;
+    __syncthreads();  // (the scan's partial sums are read before they are written again)
+  }
+  if (threadIdx.x == 0) hist[static_cast<size_t>(blocks) * ids + blockIdx.x] = before;
+}
+
+__global__ void __launch_bounds__(kGroupThreads) group_place_kernel(GroupArgs a, int blocks, const int32_t* hist,
+                                                                    bool summed) {
+  __shared__ GroupShared s;
+  group_block(a, blockIdx.x, blocks, hist, summed, s);
 }
 
 template <int WPR>
 hipError_t launch_group(const GroupArgs& a, int32_t* hist, hipStream_t stream) {
-  const int blocks = std::max(1, (a.numel + kGroupRoutes - 1) / kGroupRoutes);
+  const int blocks = std::max(1, group_blocks(a.numel));
   const int quant = WPR ? (a.x_rows * WPR + kGroupWaves - 1) / kGroupWaves : 0;
   constexpr auto one = group_routes_kernel<WPR>;
   constexpr auto count = group_count_kernel<WPR>;
@@ -178,8 +216,12 @@ hipError_t launch_group(const GroupArgs& a, int32_t* hist, hipStream_t stream) {
     hipLaunchKernelGGL(one, dim3(1 + quant), dim3(kGroupThreads), 0, stream, a);
   } else {
     hipLaunchKernelGGL(count, dim3(blocks + quant), dim3(kGroupThreads), 0, stream, a, blocks, hist);
+    const bool summed = group_sums(blocks, a.num_experts);
+    if (summed)
+      hipLaunchKernelGGL(group_sum_kernel, dim3(a.num_experts + 1), dim3(kGroupThreads), 0, stream, a.num_experts + 1,
+                         blocks, hist);
     hipLaunchKernelGGL(group_place_kernel, dim3(blocks), dim3(kGroupThreads), 0, stream, a, blocks,
-                       static_cast<const int32_t*>(hist));
+                       static_cast<const int32_t*>(hist), summed);
   }
   return hipGetLastError();
 }
@@ -187,8 +229,8 @@ hipError_t launch_group(const GroupArgs& a, int32_t* hist, hipStream_t stream) {
 }  // namespace
 
 size_t group_hist_ints(int numel, int num_experts) {
-  const size_t blocks = (static_cast<size_t>(numel) + kGroupRoutes - 1) / kGroupRoutes;
-  return blocks > 1 ? blocks * (num_experts + 1) : 0;
+  const int blocks = group_blocks(numel);
+  return blocks > 1 ? (blocks + static_cast<size_t>(group_sums(blocks, num_experts))) * (num_experts + 1) : 0;
 }
 
 hipError_t launch_group_routes(const GroupArgs& a, int32_t* hist, hipStream_t stream) {

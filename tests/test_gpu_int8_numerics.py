@@ -298,3 +298,31 @@ def test_layer_of_more_tokens_than_a_launch(dev):
     for first in (0, (1 << 23) - 50, M - 100):
         part = slice(first, first + 100)
         assert torch.equal(y[part], ops.experts_int8(x[part], tw[part], ids[part], bank, route_dtype=torch.float32))
+
+
+@pytest.mark.parametrize("E", [1, 16, 1023])
+@pytest.mark.parametrize("numel", [2048 * 63 + 1, 2048 * 64 - 1, 2048 * 65, 1_200_001, 2048 * 1025 + 3, 30_000_000])
+def test_group_routes_long(dev, numel, E):
+    """Long lists of routes: stable, with ids of no expert left out and the tail filled."""
+    ids = torch.randint(-2, E + 3, (numel,), generator=gen(dev, numel + E), device=dev, dtype=torch.int32)
+    if E > 1:
+        ids[numel // 3 : numel // 2] = E // 2  # a long run of one expert
+    order, offsets = ops.group_routes(ids, E)
+    key = torch.where((ids < 0) | (ids > E), E + 1, ids)
+    counts = torch.bincount(key, minlength=E + 2)
+    assert torch.equal(offsets.long(), torch.cat([counts.new_zeros(1), counts[:E].cumsum(0)]))
+    listed = int(counts[: E + 1].sum())
+    assert torch.equal(order[:listed].long(), torch.sort(key, stable=True).indices[:listed])
+    assert bool((order[listed:] == numel).all())
+
+
+def test_group_routes_longest(dev):
+    """The most routes that 32 bits count, few of them of an expert: the places near both ends."""
+    numel, E = (1 << 31) - 1, 5
+    ids = torch.full((numel,), -1, dtype=torch.int32, device=dev)
+    at = torch.tensor([0, 2047, 2048, 1 << 30, numel - 2049, numel - 2, numel - 1], device=dev)
+    ids[at] = torch.tensor([3, 0, 3, 4, 0, 3, 0], dtype=torch.int32, device=dev)
+    order, offsets = ops.group_routes(ids, E)
+    assert offsets.tolist() == [0, 3, 3, 3, 6, 7]
+    assert order[:7].tolist() == [2047, numel - 2049, numel - 1, 0, 2048, numel - 2, 1 << 30]
+    assert all(bool((part == numel).all()) for part in order[7:].split(1 << 28))
