@@ -976,7 +976,7 @@ int ftmoe_grouped_matmul(const ftmoe_grouped* g, ftmoe_stream_t stream) {
 
 size_t ftmoe_experts_int8_rows_workspace(int M, int top_k, const ftmoe_bank* bank, const ftmoe_bank* shared,
                                          int route_dtype) {
-  if (!bank || M <= 0 || top_k <= 0) return 0;
+  if (!bank || M <= 0 || top_k <= 0 || static_cast<long long>(M) * top_k + M > INT32_MAX) return 0;
   return int8_layout(nullptr, M, top_k, bank, shared, route_dtype).bytes;
 }
 
@@ -1002,7 +1002,7 @@ int ftmoe_experts_int8_rows(const void* x, int M, int top_k, const float* topk_w
     if (shared->hidden != bank->hidden)
       return fail(FTMOE_ERR_INVALID, "shared hidden %d != %d", shared->hidden, bank->hidden);
   }
-  if (M < 0 || top_k <= 0 || static_cast<long long>(M) * top_k > INT32_MAX)
+  if (M < 0 || top_k <= 0 || static_cast<long long>(M) * top_k + M > INT32_MAX)  // (M rows of the shared expert)
     return fail(FTMOE_ERR_INVALID, "experts_int8: M=%d top_k=%d", M, top_k);
   if (activation < FTMOE_ACT_SILU || activation > FTMOE_ACT_GELU_TANH)
     return fail(FTMOE_ERR_UNSUPPORTED, "experts_int8: activation %d", activation);

@@ -320,6 +320,12 @@ def _launch(what: str, fn, dev: torch.device, *args) -> None:
         check(rc, what)
 
 
+def _check_int32(what: str, *sizes: int) -> None:
+    """Sizes go to the library as 32-bit integers, and larger ones would arrive cut."""
+    if max(sizes) > 0x7FFFFFFF:
+        raise ValueError(f"{what}: a size of {max(sizes)} passes 32 bits")
+
+
 def _act_code(activation: str | None) -> int:
     if activation is None:
         return _lib.ACT_NONE
@@ -337,8 +343,9 @@ def act_quant_int8(x: torch.Tensor):
         raise ValueError("x must be bfloat16")
     if x.dim() < 1:
         raise ValueError("x must have rows")
-    dev = _one_gpu(x)
     *lead, k = x.shape
+    _check_int32("act_quant_int8", math.prod(lead), k)
+    dev = _one_gpu(x)
     q = torch.empty_like(x, dtype=torch.int8)  # (1 us less than torch.empty of the shape)
     s = torch.empty(lead, dtype=torch.float32, device=dev)
     _launch("act_quant_int8", lib().ftmoe_act_quant_int8, dev, x.data_ptr(), s.numel(), k, q.data_ptr(), s.data_ptr())
@@ -362,6 +369,7 @@ def matmul_int8(q: torch.Tensor, q_scale: torch.Tensor, w: torch.Tensor, w_scale
         raise ValueError("scales must be float32")
     if q_scale.shape != (m,) or w_scale.shape != (n,):
         raise ValueError("one scale per row of q and of w")
+    _check_int32("matmul_int8", m, n, k)
     act = _act_code(activation)
     dev = _one_gpu(q, q_scale, w, w_scale, out)
     shape = (m, n if activation is None else n // 2)
@@ -384,7 +392,9 @@ def group_routes(topk_ids: torch.Tensor, num_experts: int):
     among those positions."""
     if topk_ids.dtype != torch.int32:
         raise ValueError("topk_ids must be int32")
-    dev, numel = _one_gpu(topk_ids), topk_ids.numel()
+    numel = topk_ids.numel()
+    _check_int32("group_routes", numel, num_experts)
+    dev = _one_gpu(topk_ids)
     order = torch.empty((numel,), dtype=torch.int32, device=dev)
     offsets = torch.empty((max(num_experts, 0) + 2,), dtype=torch.int32, device=dev)
     ws = torch.empty((lib().ftmoe_group_routes_workspace(numel, num_experts),), dtype=torch.uint8, device=dev)
@@ -415,6 +425,7 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, orde
         raise ValueError("top_k is 1 without an order, else positive")
     (t, k), (e, n) = x.shape, w.shape[:2]
     rows = t * top_k
+    _check_int32("grouped_matmul", t, rows, e, n, k)
     if offsets.dtype != torch.int32 or tuple(offsets.shape) != (e + 1,):
         raise ValueError("offsets must be int32 [experts + 1]")
     if order is not None and (order.dtype != torch.int32 or order.numel() != rows):
@@ -756,6 +767,7 @@ def experts_int8(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.Tensor, 
         raise ValueError(f"Unsupported activation: {activation}")
     if bank.fmt != "int8" or (shared is not None and shared.fmt != "int8"):
         raise ValueError("experts_int8 takes int8 banks")
+    _check_int32("experts_int8", topk_ids.numel(), bank.hidden, 2 * bank.inter, shared.inter if shared is not None else 0)
     if route_dtype not in (torch.bfloat16, torch.float32):
         raise ValueError("the routes' rows are bfloat16 or float32")
     dev = _one_gpu(x, topk_w, topk_ids, out, bank.gate_up, bank.down, bank.gate_up_scale, bank.down_scale,

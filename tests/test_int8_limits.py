@@ -43,3 +43,43 @@ def test_most_features():
     for fmt in (_lib.FMT_INT8, _lib.FMT_BF16):
         g = _lib.FtmoeGrouped(fmt, 1, n, 16, 4096, 4096, 4096, 4096, 1, 1, 4096, None, None, -1, 4096)
         assert L.ftmoe_grouped_matmul(ctypes.byref(g), None) == UNSUPPORTED
+
+
+def test_workspace_of_routes_past_32_bits():
+    """No size that a caller would allocate: the call refuses."""
+    L = _lib.lib()
+    bank = _lib.FtmoeBank(_lib.FMT_INT8, 8, 64, 32, 16, 16, 16, 16)
+    bp = ctypes.byref(bank)
+    for M, k in [(1 << 20, 1 << 12), (1 << 30, 1), (1 << 27, 33), ((1 << 31) - 1, 1)]:
+        assert L.ftmoe_experts_int8_workspace(M, k, bp, None) == 0
+        assert L.ftmoe_experts_int8(P, M, k, P, P, bp, None, 0, P, P, 1 << 60, None) == INVALID
+
+
+def test_wrappers_refuse_sizes_past_32_bits():
+    """They would reach the library cut to 32 bits: 2^32 + 4 rows as 4."""
+    big = (1 << 32) + 16
+
+    def many(*shape, dtype=torch.int8):
+        return torch.zeros((1,) * len(shape), dtype=dtype).expand(*shape)
+
+    f32, i32, bf16 = torch.float32, torch.int32, torch.bfloat16
+    for call in [
+        lambda: ops.act_quant_int8(many(big, 16, dtype=bf16)),
+        lambda: ops.act_quant_int8(many(1 << 16, (1 << 16) + 1, 16, dtype=bf16)),
+        lambda: ops.act_quant_int8(many(2, big, dtype=bf16)),
+        lambda: ops.matmul_int8(many(big, 16), many(big, dtype=f32), many(8, 16), many(8, dtype=f32)),
+        lambda: ops.matmul_int8(many(4, 16), many(4, dtype=f32), many(big, 16), many(big, dtype=f32)),
+        lambda: ops.matmul_int8(many(4, big), many(4, dtype=f32), many(8, big), many(8, dtype=f32)),
+        lambda: ops.group_routes(many(big, dtype=i32), 8),
+        lambda: ops.group_routes(many(8, dtype=i32), big),
+        lambda: ops.grouped_matmul(many(big, 16, dtype=bf16), many(2, 8, 16, dtype=bf16), many(3, dtype=i32)),
+        lambda: ops.grouped_matmul(many(4, 16, dtype=bf16), many(2, big, 16, dtype=bf16), many(3, dtype=i32)),
+        lambda: ops.grouped_matmul(many(4, 16, dtype=bf16), many(2, 8, 16, dtype=bf16), many(3, dtype=i32),
+                                   order=many(4 << 30, dtype=i32), top_k=1 << 30),
+        lambda: ops.grouped_matmul(many(4, big, dtype=bf16), many(2, 8, big, dtype=bf16), many(3, dtype=i32)),
+        lambda: ops.experts_int8(many(big, 16, dtype=bf16), many(big, 1, dtype=f32), many(big, 1, dtype=i32),
+                                 ops.ExpertBank("int8", many(2, 32, 16), many(2, 16, 16), many(2, 32, dtype=f32),
+                                                many(2, 16, dtype=f32))),
+    ]:
+        with pytest.raises(ValueError, match="32 bits"):
+            call()
