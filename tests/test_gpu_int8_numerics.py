@@ -16,7 +16,7 @@ from freetoken_amd import ops
 from freetoken_amd.layers.moe import MoELayer
 from freetoken_amd.moe.fused_int8 import fused_experts_int8
 
-from test_gpu_int8 import BF16, F32, gen, int8_rows, make_bank, routing, scales, within
+from test_gpu_int8 import BF16, F32, gen, grouped_ref, int8_rows, make_bank, routing, scales, within
 
 pytestmark = pytest.mark.gpu
 
@@ -326,3 +326,38 @@ def test_group_routes_longest(dev):
     assert offsets.tolist() == [0, 3, 3, 3, 6, 7]
     assert order[:7].tolist() == [2047, numel - 2049, numel - 1, 0, 2048, numel - 2, 1 << 30]
     assert all(bool((part == numel).all()) for part in order[7:].split(1 << 28))
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("counts", [[3, 0, 1], [70, 5, 0, 129], [300, 700]], ids=range(3))
+@pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
+def test_grouped_activation_with_weights(dev, counts, int8, act):
+    """An activation and row weights together, in a routed order: row_weight * act(gate) * up."""
+    E, R, N, K = len(counts), sum(counts), 140, 272
+    g = gen(dev, R)
+    if int8:
+        x, w, xs, ws = int8_rows(dev, g, R, K), int8_rows(dev, g, E, N, K), scales(dev, g, R), scales(dev, g, E, N)
+    else:
+        x = torch.randn((R, K), generator=g, device=dev).to(torch.bfloat16)
+        w, xs, ws = torch.randn((E, N, K), generator=g, device=dev).mul_(0.1).to(torch.bfloat16), None, None
+    weight = torch.randn(R, generator=g, device=dev)
+    order = torch.randperm(R, generator=g, device=dev).to(torch.int32)
+    offsets = torch.tensor([0] + counts, dtype=torch.int32, device=dev).cumsum(0, dtype=torch.int32)
+    y = ops.grouped_matmul(x, w, offsets, order=order, x_scale=xs, w_scale=ws, row_weight=weight, activation=act)
+    at = order.long()
+    ref, err = grouped_ref(x, w, counts, (at, at), act, weight, xs, ws)
+    within(y, ref, err)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("M,k,E,H,I", [(1, 8, 128, 2048, 768), (4, 2, 16, 1024, 512), (2, 4, 16, 4096, 512)])
+def test_small_steps_with_every_activation(dev, M, k, E, H, I, act):
+    """Steps that quantise inside the products give the operators' results one by one, whatever the activation."""
+    g = gen(dev, M + H)
+    bank = make_bank(dev, g, E, H, I)
+    x = torch.randn((M, H), generator=g, device=dev).to(torch.bfloat16)
+    tw, ids = routing(dev, g, M, k, E)
+    y = ops.experts_int8(x, tw, ids, bank, activation=act, route_dtype=torch.float32)
+    rows = down_rows(*activations(x, ids, bank, act), ids, bank, tw)
+    ref, off = rows.sum(1), rows.abs().sum(1) * (F32 + (k + 1) * 2.0**-24)
+    within(y, ref, off + (ref.abs() + off) * BF16)
