@@ -320,10 +320,11 @@ def _launch(what: str, fn, dev: torch.device, *args) -> None:
         check(rc, what)
 
 
-def _check_int32(what: str, *sizes: int) -> None:
-    """Sizes go to the library as 32-bit integers, and larger ones would arrive cut."""
-    if max(sizes) > 0x7FFFFFFF:
-        raise ValueError(f"{what}: a size of {max(sizes)} passes 32 bits")
+def _check_int32(what: str, sizes: int) -> None:
+    """Sizes go to the library as 32-bit integers, and larger ones would arrive cut (``sizes``: any of them, joined
+    by ``|``)."""
+    if sizes >> 31:
+        raise ValueError(f"{what}: a size passes 32 bits")
 
 
 def _act_code(activation: str | None) -> int:
@@ -344,7 +345,7 @@ def act_quant_int8(x: torch.Tensor):
     if x.dim() < 1:
         raise ValueError("x must have rows")
     *lead, k = x.shape
-    _check_int32("act_quant_int8", math.prod(lead), k)
+    _check_int32("act_quant_int8", math.prod(lead) | k)
     dev = _one_gpu(x)
     q = torch.empty_like(x, dtype=torch.int8)  # (1 us less than torch.empty of the shape)
     s = torch.empty(lead, dtype=torch.float32, device=dev)
@@ -369,7 +370,7 @@ def matmul_int8(q: torch.Tensor, q_scale: torch.Tensor, w: torch.Tensor, w_scale
         raise ValueError("scales must be float32")
     if q_scale.shape != (m,) or w_scale.shape != (n,):
         raise ValueError("one scale per row of q and of w")
-    _check_int32("matmul_int8", m, n, k)
+    _check_int32("matmul_int8", m | n | k)
     act = _act_code(activation)
     dev = _one_gpu(q, q_scale, w, w_scale, out)
     shape = (m, n if activation is None else n // 2)
@@ -393,7 +394,7 @@ def group_routes(topk_ids: torch.Tensor, num_experts: int):
     if topk_ids.dtype != torch.int32:
         raise ValueError("topk_ids must be int32")
     numel = topk_ids.numel()
-    _check_int32("group_routes", numel, num_experts)
+    _check_int32("group_routes", numel | max(num_experts, 0))
     dev = _one_gpu(topk_ids)
     order = torch.empty((numel,), dtype=torch.int32, device=dev)
     offsets = torch.empty((max(num_experts, 0) + 2,), dtype=torch.int32, device=dev)
@@ -425,7 +426,7 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, orde
         raise ValueError("top_k is 1 without an order, else positive")
     (t, k), (e, n) = x.shape, w.shape[:2]
     rows = t * top_k
-    _check_int32("grouped_matmul", t, rows, e, n, k)
+    _check_int32("grouped_matmul", rows | e | n | k)
     if offsets.dtype != torch.int32 or tuple(offsets.shape) != (e + 1,):
         raise ValueError("offsets must be int32 [experts + 1]")
     if order is not None and (order.dtype != torch.int32 or order.numel() != rows):
@@ -499,6 +500,7 @@ class ExpertBank:
             rows, hidden, inter = self.down.shape
             if tuple(self.gate_up.shape) != (rows, 2 * inter, hidden):
                 raise ValueError("int8 bank matrices are [rows, 2 inter, hidden] and [rows, hidden, inter]")
+            _check_int32("int8 bank", rows | hidden | 2 * inter)
 
     @property
     def num_rows(self) -> int:
@@ -747,6 +749,9 @@ def quantize_bank_int8(bank: ExpertBank) -> ExpertBank:
     return ExpertBank("int8", gate_up, down, gs, ds, swiglu_limit=bank.swiglu_limit)
 
 
+_ROW_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
+
+
 def experts_int8(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.Tensor, bank: ExpertBank,
                  shared: ExpertBank | None = None, activation: str = "silu",
                  out: torch.Tensor | None = None, route_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -767,8 +772,9 @@ def experts_int8(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.Tensor, 
         raise ValueError(f"Unsupported activation: {activation}")
     if bank.fmt != "int8" or (shared is not None and shared.fmt != "int8"):
         raise ValueError("experts_int8 takes int8 banks")
-    _check_int32("experts_int8", topk_ids.numel(), bank.hidden, 2 * bank.inter, shared.inter if shared is not None else 0)
-    if route_dtype not in (torch.bfloat16, torch.float32):
+    _check_int32("experts_int8", topk_ids.numel())
+    rows = _ROW_DTYPES.get(route_dtype)
+    if rows is None:
         raise ValueError("the routes' rows are bfloat16 or float32")
     dev = _one_gpu(x, topk_w, topk_ids, out, bank.gate_up, bank.down, bank.gate_up_scale, bank.down_scale,
                    *((shared.gate_up, shared.down, shared.gate_up_scale, shared.down_scale) if shared else ()))
@@ -784,7 +790,6 @@ def experts_int8(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.Tensor, 
     bp = ctypes.byref(b)
     sp = ctypes.byref(sb) if sb is not None else None
     # a workspace of the call's own: of the stream's pool, or of the graph's under capture
-    rows = _lib.DTYPE_F32 if route_dtype == torch.float32 else _lib.DTYPE_BF16
     ws = torch.empty((lib().ftmoe_experts_int8_rows_workspace(m, k, bp, sp, rows),), dtype=torch.uint8, device=dev)
     y = out if out is not None else torch.empty_like(x)
     _launch("experts_int8", lib().ftmoe_experts_int8_rows, dev, _ptr(x), m, k, _ptr(topk_w), _ptr(topk_ids), bp, sp,

@@ -80,6 +80,9 @@ def test_wrappers_refuse_sizes_past_32_bits():
         lambda: ops.experts_int8(many(big, 16, dtype=bf16), many(big, 1, dtype=f32), many(big, 1, dtype=i32),
                                  ops.ExpertBank("int8", many(2, 32, 16), many(2, 16, 16), many(2, 32, dtype=f32),
                                                 many(2, 16, dtype=f32))),
+        lambda: ops.ExpertBank("int8", many(2, 32, big), many(2, big, 16), many(2, 32, dtype=f32), many(2, big, dtype=f32)),
+        lambda: ops.ExpertBank("int8", many(2, 1 << 31, 16), many(2, 16, 1 << 30), many(2, 1 << 31, dtype=f32),
+                               many(2, 16, dtype=f32)),
     ]:
         with pytest.raises(ValueError, match="32 bits"):
             call()
