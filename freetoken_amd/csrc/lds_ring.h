@@ -1,5 +1,5 @@
 // Pieces of the GEMMs whose operands come through a ring of LDS stages by direct
-// global -> LDS copies (prefill.hip, matmul.hip): explicit waits and barriers, the
+// global -> LDS copies (prefill.hip, matmul_stream.hip, matmul_tile.hip): explicit waits and barriers, the
 // copies, the LDS swizzle and the tiles' order.
 #pragma once
 

@@ -1,4 +1,5 @@
-// Pieces shared by the matrix products' kernels (matmul.hip, matmul_tile.hip).
+// Pieces shared by the matrix products' kernels (matmul.hip, matmul_stream.hip, matmul_tile.hip) and the grouping of
+// routes (group.hip).
 #pragma once
 
 #include "kernels.h"

@@ -37,7 +37,7 @@ __device__ __forceinline__ void add_row8(float (&acc)[8], const u32x4 (&v)[sizeo
 // y[t] = bf16(sum of the routes' rows in route order, then the shared row M k + t),
 // routes with ids outside [0, num_rows) skipped; H a multiple of 8; rows of T, bf16 (uint16_t) or float32.
 // The rows of eight routes are read before the first is added.  Bound by reading them: 8192 x 8
-// rows of 2048 bf16 49 us (6.1 TB/s, part of it from the memory-side cache).
+// rows of 2048 bf16 49 us (6.1 TB/s, part of it from the memory-side cache), float32 101 (5.7 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(kCombineThreads) combine_routes_kernel(const T* __restrict__ routes,
                                                                          const int32_t* __restrict__ ids, int num_rows,

@@ -7,9 +7,11 @@
 // wave copies its weight lines global -> LDS by LDS-DMA into a ring of its own (no
 // barrier in the K loop): an instruction covers 8 whole 128-byte lines, where a
 // register load in the operand layout covers half lines.  x comes straight to registers.
-// Three stages of 2 KB a wave (4 with gate and up rows): five workgroups (three) fit a
-// CU, and 120 KB (144) of weights are on their way to it.  Measured: 512 rows over 128 experts, N 1536 (gate and up), K 2048,
-// 61 us (6.6 TB/s of weights), 8 rows 9.1 us (2.8 TB/s: latency of one short pass).
+// Three stages of 2 KB a wave (4 with gate and up rows), two of them on their way while the third is multiplied: where
+// there are enough workgroups six (three) of them share a CU, with 144 KB of LDS and 96 KB of weights on their way.
+// Where there are not (one row, N 4096: one a CU) it is 16 KB, and latency bounds the call.  Measured: 512 rows over
+// 128 experts, N 1536 (gate and up), K 2048, 61 us (6.6 TB/s of weights), 8 rows 9.1 us (2.8 TB/s: latency of one short
+// pass).
 //
 // QX: x is bf16.  The workgroup quantises its rows (quant_int8.h, the codes that
 // act_quant_int8 gives) into LDS while its first weights are on their way, which saves

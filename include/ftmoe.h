@@ -404,7 +404,8 @@ int ftmoe_experts_int8(const void* x, int M, int top_k, const float* topk_w, con
                        const ftmoe_bank* bank, const ftmoe_bank* shared, int activation, void* y, void* workspace,
                        size_t workspace_bytes, ftmoe_stream_t stream);
 /* The same with the routes' rows (and the shared expert's) in route_dtype:
- * FTMOE_DTYPE_BF16 as above, or FTMOE_DTYPE_F32: then only y is rounded. */
+ * FTMOE_DTYPE_BF16 as above, or FTMOE_DTYPE_F32: then y is the only rounding
+ * after the activations. */
 size_t ftmoe_experts_int8_rows_workspace(int M, int top_k, const ftmoe_bank* bank, const ftmoe_bank* shared,
                                          int route_dtype);
 int ftmoe_experts_int8_rows(const void* x, int M, int top_k, const float* topk_w, const int32_t* topk_ids,
