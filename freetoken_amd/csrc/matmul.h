@@ -56,7 +56,7 @@ struct RowFactor {
   float first, last;
 };
 __device__ __forceinline__ RowFactor row_factor(float scale) {
-  return scale < 1.0f ? RowFactor{scale, 1.0f} : RowFactor{1.0f, scale};
+  return fabsf(scale) < 1.0f ? RowFactor{scale, 1.0f} : RowFactor{1.0f, scale};
 }
 __device__ __forceinline__ float scaled(float sum, const RowFactor& x, float ws) { return sum * x.first * ws * x.last; }
 

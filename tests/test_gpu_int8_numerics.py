@@ -213,6 +213,7 @@ def test_far_scales(dev, M, top, wtop):
     assert int(normal.sum()) >= normal.numel() // 2
     y = ops.matmul_int8(q, s, w, ws, out_dtype=torch.float32)
     within(torch.where(normal, y.double(), 0.0), torch.where(normal, ref, 0.0), ref.abs() * F32)
+    assert torch.equal(ops.matmul_int8(q, -s, w, ws, out_dtype=torch.float32), -y)  # a scale's sign is its own
     offsets = torch.tensor([0, M], dtype=torch.int32, device=dev)
     weight = torch.rand(M, generator=g, device=dev)
     y = ops.grouped_matmul(q, w[None], offsets, x_scale=s, w_scale=ws[None], row_weight=weight)
